@@ -223,7 +223,8 @@ def _plain_grouped(s):
 def _plain_quantize(x):
     v = x.float()
     largest = v.abs().amax(dim=1).clamp_min(2.0**-100)
-    q = torch.round(v * (127.0 / largest)[:, None]).to(torch.int8)
+    # (A number divided by a tensor is its reciprocal times the number: rounded twice.)
+    q = torch.round(v * (torch.full_like(largest, 127.0) / largest)[:, None]).to(torch.int8)
     return [q, largest / 127.0]
 
 
