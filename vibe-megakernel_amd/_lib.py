@@ -1,4 +1,5 @@
-"""ctypes binding of the C ABI in include/megamoe.h (libmegamoe.so, built in-tree).
+"""ctypes binding of the C ABI in include/megamoe.h and include/megamoe_products.h
+(libmegamoe.so, built in-tree).
 
 There is no fallback: if the shared library is missing or cannot be loaded,
 ``load()`` raises, so nothing on the product path can silently run elsewhere.
@@ -28,6 +29,12 @@ SYMBOLS = ("megamoe_workspace_bytes", "megamoe_forward", "megamoe_forward_events
            "megamoe_layer_forward", "megamoe_layer_status", "megamoe_mx_layer_forward", "megamoe_mx_layer_status",
            "megamoe_e4m3_selftest", "megamoe_forward_w8a16", "megamoe_layer_forward_w8a16")
 ABI_VERSION = 11
+
+# The functions of megamoe_products.h.
+PRODUCT_SYMBOLS = ("megamoe_grouped_mm", "megamoe_grouped_mm_wgrad", "megamoe_int8_mm", "megamoe_quantize_rows_int8",
+                   "megamoe_products_version")
+PRODUCTS_VERSION = 1
+BF16, FP16, FP32 = range(3)  # enum megamoe_product_type
 
 
 class Desc(ctypes.Structure):
@@ -69,6 +76,12 @@ EP_SEND_FIELDS = ("rows", "row_scales", "ids", "weights", "counts", "slot_rows")
 
 class EpSend(ctypes.Structure):
     _fields_ = [(name, ctypes.c_void_p) for name in EP_SEND_FIELDS]
+
+
+class Product(ctypes.Structure):
+    _fields_ = [("rows", ctypes.c_int64), ("groups", ctypes.c_int32), ("n", ctypes.c_int32), ("k", ctypes.c_int32),
+                ("dtype", ctypes.c_int32), ("transposed", ctypes.c_int32), ("fill_rest", ctypes.c_int32),
+                ("ldx", ctypes.c_int64), ("ldy", ctypes.c_int64)]
 
 
 class MegaMoEError(RuntimeError):
@@ -120,7 +133,13 @@ def load() -> ctypes.CDLL:
     lib.megamoe_status_string.argtypes = [c_int]
     lib.megamoe_status_string.restype = ctypes.c_char_p
     lib.megamoe_abi_version.argtypes = []
-    for name in SYMBOLS:
+    lib.megamoe_grouped_mm.argtypes = [P(Product), c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]
+    lib.megamoe_grouped_mm_wgrad.argtypes = [P(Product), c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]
+    lib.megamoe_int8_mm.argtypes = [P(Product), c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]
+    lib.megamoe_quantize_rows_int8.argtypes = [ctypes.c_int64, ctypes.c_int32, ctypes.c_int64, ctypes.c_int32, c_void_p,
+                                               c_void_p, c_void_p, c_void_p]
+    lib.megamoe_products_version.argtypes = []
+    for name in SYMBOLS + PRODUCT_SYMBOLS:
         if name != "megamoe_status_string":
             getattr(lib, name).restype = c_int
     _lib = lib

@@ -11,17 +11,19 @@ import json
 import os
 import re
 import subprocess
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PACKAGE_DIR = Path(__file__).resolve().parent
 REPO = PACKAGE_DIR.parent
-SOURCE = PACKAGE_DIR / "csrc" / "megamoe.hip"
+SOURCES = (PACKAGE_DIR / "csrc" / "megamoe.hip", PACKAGE_DIR / "csrc" / "products.hip")
 OUTPUT = PACKAGE_DIR / "libmegamoe.so"
 REPORT = PACKAGE_DIR / "libmegamoe.kernels.json"
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
 FLAGS = [
-    "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared",
+    "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC",
     # Rounding points are written explicitly; no implicit fused multiply-add.
     "-ffp-contract=off",
     # No packed fp32 VALU instructions.
@@ -58,19 +60,38 @@ def resource_report(stderr: str) -> dict:
     return out
 
 
+def _finish(procs: list) -> list[str]:
+    """The compilers' messages, once all have ended; raises if one failed."""
+    with ThreadPoolExecutor(len(procs)) as pool:  # both pipes are drained while both compile
+        logs = list(pool.map(lambda p: p.communicate()[1], procs))
+    for proc, log in zip(procs, logs):
+        if proc.returncode != 0:
+            raise RuntimeError(f"hipcc failed ({proc.returncode}):\n{log}")
+    return logs
+
+
 def build_library(verbose: bool = False, defines: tuple[str, ...] = (), output: Path | None = None) -> Path:
     """Builds the library (``output``: another path, for a check build with ``defines``, e.g.
     ``MEGAMOE_AGENT_ACQUIRE=1``; its resource report is not kept)."""
     out = OUTPUT if output is None else Path(output)
     tmp = out.with_suffix(".so.tmp")
-    cmd = [HIPCC, *FLAGS, *[f"-D{d}" for d in defines], f"-I{REPO / 'include'}", str(SOURCE), "-o", str(tmp)]
-    proc = subprocess.run(cmd, capture_output=True, text=True)
-    if proc.returncode != 0:
-        raise RuntimeError(f"hipcc failed ({proc.returncode}):\n{proc.stderr}")
-    other = [l for l in proc.stderr.splitlines() if "kernel-resource-usage" not in l]
+    with tempfile.TemporaryDirectory(prefix="megamoe_build_") as objects:
+        # The sources share nothing but headers: compiled side by side, then linked.
+        parts = [(src, Path(objects) / (src.stem + ".o")) for src in SOURCES]
+        procs = [subprocess.Popen([HIPCC, *FLAGS, *[f"-D{d}" for d in defines], f"-I{REPO / 'include'}", "-c",
+                                   str(src), "-o", str(obj)], stdout=subprocess.DEVNULL, stderr=subprocess.PIPE,
+                                  text=True) for src, obj in parts]
+        logs = _finish(procs)
+        link = subprocess.run([HIPCC, "--offload-arch=gfx950", "-shared", *[str(obj) for _, obj in parts], "-o",
+                               str(tmp)], capture_output=True, text=True)
+        if link.returncode != 0:
+            raise RuntimeError(f"hipcc failed to link ({link.returncode}):\n{link.stderr}")
+    other = [l for log in logs for l in log.splitlines() if "kernel-resource-usage" not in l]
     if verbose and any(l.strip() for l in other):
         print("\n".join(other))
-    report = resource_report(proc.stderr)
+    report = {}
+    for log in logs:
+        report.update(resource_report(log))
     if not report:
         raise RuntimeError("hipcc printed no kernel resource report")
     if output is None:

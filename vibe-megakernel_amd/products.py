@@ -1,0 +1,250 @@
+"""The experts' matrix products outside the fused layer (include/megamoe_products.h).
+
+``submission.MoELayer`` runs routing, experts and combine in one launch, with E4M3 or MXFP4
+experts. These are the products by themselves, for programs that bring the rows into expert
+order on their own: to train or adapt experts in bf16 or fp16 (``grouped_mm``, differentiable),
+and to serve experts held in int8 with one scale for each token and each output channel
+(``quantize_rows_int8``, ``grouped_int8_mm``, and ``int8_mm`` for a single matrix such as a
+shared expert's).
+
+``counts`` (int64 [E], on the GPU) holds the rows of each expert, in order: expert e's rows
+start where expert e-1's end. It is read on the device only, so no call waits for the host.
+Rows behind the last expert's belong to none: their results are zero, or stay as they were in
+``out``. Counts that are negative or add up to more than the rows make the whole result NaN.
+
+Every call is issued on torch's current stream of the inputs' device, as one kernel without a
+workspace, and can be captured in a graph after the same call ran once outside. There is no
+fallback; bad arguments raise ValueError, tensors off the GPU RuntimeError, a failed launch or
+a geometry beyond the limits MegaMoEError.
+"""
+
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _lib
+from .submission import _on, _stream_handle
+
+_TYPES = {torch.bfloat16: _lib.BF16, torch.float16: _lib.FP16, torch.float32: _lib.FP32}
+_byref = ctypes.byref
+
+
+def _device(t, name: str) -> torch.device:
+    if not isinstance(t, torch.Tensor):
+        raise ValueError(f"{name}: expected a tensor")
+    if t.device.type != "cuda":
+        raise RuntimeError(f"the products run on a GPU; {name} is on {t.device}")
+    return t.device
+
+
+def _dense(t, name: str, dtype, shape, device) -> None:
+    if not isinstance(t, torch.Tensor):
+        raise ValueError(f"{name}: expected a tensor")
+    if t.dtype != dtype or tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name}: expected {tuple(shape)} {dtype}, got {tuple(t.shape)} {t.dtype}")
+    if t.device != device or not t.is_contiguous():
+        raise ValueError(f"{name}: must be contiguous on {device}")
+
+
+def _stride(t: torch.Tensor) -> int | None:
+    """The row stride of 2-D ``t``, or None if its rows are not dense or overlap."""
+    rows, cols = t.shape
+    if cols > 1 and t.stride(1) != 1:
+        return None
+    if rows <= 1:
+        return max(cols, 1)
+    return t.stride(0) if t.stride(0) >= cols else None
+
+
+def _rows(t, name: str, dtype, cols, device) -> tuple[torch.Tensor, int]:
+    """2-D input rows and their stride; rows that are not dense (a broadcast or transposed
+    tensor) are copied."""
+    if not isinstance(t, torch.Tensor):
+        raise ValueError(f"{name}: expected a tensor")
+    if t.dim() != 2 or t.dtype != dtype or (cols is not None and t.shape[1] != cols):
+        raise ValueError(f"{name}: expected [rows, {'columns' if cols is None else cols}] {dtype}, "
+                         f"got {tuple(t.shape)} {t.dtype}")
+    if t.device != device:
+        raise ValueError(f"{name}: on {t.device}, expected {device}")
+    ld = _stride(t)
+    if ld is None:
+        t = t.contiguous()
+        ld = max(t.shape[1], 1)
+    return t, ld
+
+
+def _extent(t: torch.Tensor) -> tuple[int, int]:
+    """The bytes [first, last) that ``t`` spans."""
+    if t.numel() == 0:
+        return 0, 0
+    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+
+def _result(out, shape, dtype, device, inputs) -> tuple[torch.Tensor, int]:
+    """The result's tensor and row stride; a given ``out`` may not overlap an input."""
+    if out is None:
+        return torch.empty(shape, dtype=dtype, device=device), max(shape[-1], 1)
+    if not isinstance(out, torch.Tensor):
+        raise ValueError("out: expected a tensor")
+    if out.dtype != dtype or tuple(out.shape) != tuple(shape) or out.device != device:
+        raise ValueError(f"out: expected {tuple(shape)} {dtype} on {device}, got {tuple(out.shape)} {out.dtype} on "
+                         f"{out.device}")
+    ld = _stride(out) if out.dim() == 2 else (max(shape[-1], 1) if out.is_contiguous() else None)
+    if ld is None:
+        raise ValueError("out: its rows must be dense and apart")
+    if torch.is_grad_enabled() and out.requires_grad:
+        raise ValueError("out: must not require a gradient")
+    a, b = _extent(out)
+    for t in inputs:
+        c, d = _extent(t)
+        if a < d and c < b:
+            raise ValueError("out: overlaps an input")
+    return out, ld
+
+
+def _run(fn, what: str, device: torch.device, *args) -> None:
+    stream = _stream_handle(device)
+    with _on(device):
+        status = fn(*args, stream)
+    if status:
+        _lib.check(status, what)
+
+
+def _grouped(x, weight, counts, transposed: bool, out) -> torch.Tensor:
+    device = _device(x, "x")
+    if x.dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError(f"x: expected bfloat16 or float16, got {x.dtype}")
+    if not isinstance(weight, torch.Tensor) or weight.dim() != 3:
+        raise ValueError("weight: expected [experts, out, in] (or [experts, in, out] when transposed)")
+    E = weight.shape[0]
+    N, K = (weight.shape[2], weight.shape[1]) if transposed else weight.shape[1:]
+    _dense(weight, "weight", x.dtype, weight.shape, device)
+    x, ldx = _rows(x, "x", x.dtype, K, device)
+    _dense(counts, "counts", torch.int64, (E,), device)
+    R = x.shape[0]
+    y, ldy = _result(out, (R, N), x.dtype, device, (x, weight, counts))
+    p = _lib.Product(R, E, N, K, _TYPES[x.dtype], int(transposed), int(out is None), ldx, ldy)
+    _run(_lib.load().megamoe_grouped_mm, "grouped_mm", device, _byref(p), x.data_ptr(), weight.data_ptr(),
+         counts.data_ptr(), y.data_ptr())
+    return y
+
+
+class _GroupedMM(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, counts, transposed):
+        ctx.save_for_backward(x, weight, counts)
+        ctx.transposed = transposed
+        return _grouped(x, weight, counts, transposed, None)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, weight, counts = ctx.saved_tensors
+        dx = _grouped(dy, weight, counts, not ctx.transposed, None) if ctx.needs_input_grad[0] else None
+        dw = None
+        if ctx.needs_input_grad[1]:
+            dw = grouped_mm_wgrad(x, dy, counts) if ctx.transposed else grouped_mm_wgrad(dy, x, counts)
+        return dx, dw, None, None
+
+
+def grouped_mm(x: torch.Tensor, weight: torch.Tensor, counts: torch.Tensor, *, transposed: bool = False,
+               out: torch.Tensor | None = None) -> torch.Tensor:
+    """y [R, N]: row r of expert e is ``weight[e] @ x[r]`` (weight [E, N, K]) or, ``transposed``,
+    ``x[r] @ weight[e]`` (weight [E, K, N]); bf16 or fp16, summed in fp32, rounded once.
+
+    ``x`` [R, K] may have any row stride (rows that are not dense are copied); ``weight`` is
+    dense. Differentiable in ``x`` and ``weight`` (once) unless ``out`` is given, which takes the
+    result and keeps its rows of no expert."""
+    if torch.is_grad_enabled() and ((isinstance(x, torch.Tensor) and x.requires_grad) or
+                                    (isinstance(weight, torch.Tensor) and weight.requires_grad)):
+        if out is not None:
+            raise ValueError("out: the result of inputs that require gradients cannot be written to a given tensor")
+        return _GroupedMM.apply(x, weight, counts, bool(transposed))
+    return _grouped(x, weight, counts, bool(transposed), out)
+
+
+def grouped_mm_wgrad(dy: torch.Tensor, x: torch.Tensor, counts: torch.Tensor, *,
+                     out: torch.Tensor | None = None) -> torch.Tensor:
+    """dw [E, N, K]: the gradient of ``grouped_mm``'s weight, ``dy[r]^T x[r]`` summed over each
+    expert's rows (dy [R, N], x [R, K]; exchange them for a transposed weight). Experts without
+    rows get zero."""
+    device = _device(x, "x")
+    if x.dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError(f"x: expected bfloat16 or float16, got {x.dtype}")
+    x, ldx = _rows(x, "x", x.dtype, None, device)
+    dy, ldy = _rows(dy, "dy", x.dtype, None, device)
+    if dy.shape[0] != x.shape[0]:
+        raise ValueError(f"dy: {dy.shape[0]} rows, x has {x.shape[0]}")
+    if not isinstance(counts, torch.Tensor) or counts.dim() != 1:
+        raise ValueError("counts: expected int64 [experts]")
+    E, N, K = counts.shape[0], dy.shape[1], x.shape[1]
+    _dense(counts, "counts", torch.int64, (E,), device)
+    dw, _ = _result(out, (E, N, K), x.dtype, device, (x, dy, counts))
+    p = _lib.Product(x.shape[0], E, N, K, _TYPES[x.dtype], 0, 0, ldx, ldy)
+    _run(_lib.load().megamoe_grouped_mm_wgrad, "grouped_mm_wgrad", device, _byref(p), dy.data_ptr(), x.data_ptr(),
+         counts.data_ptr(), dw.data_ptr())
+    return dw
+
+
+def _int8(x, x_scale, weight, weight_scale, counts, out_dtype, out, what: str) -> torch.Tensor:
+    device = _device(x, "x")
+    if out_dtype not in _TYPES:
+        raise ValueError(f"out_dtype: expected bfloat16, float16 or float32, got {out_dtype}")
+    K, N = weight.shape[-1], weight.shape[-2]
+    E = weight.shape[0] if counts is not None else 1
+    x, ldx = _rows(x, "x", torch.int8, K, device)
+    R = x.shape[0]
+    _dense(x_scale, "x_scale", torch.float32, (R,), device)
+    _dense(weight, "weight", torch.int8, weight.shape, device)
+    _dense(weight_scale, "weight_scale", torch.float32, weight.shape[:-1], device)
+    if counts is not None:
+        _dense(counts, "counts", torch.int64, (E,), device)
+    y, ldy = _result(out, (R, N), out_dtype, device,
+                     [t for t in (x, x_scale, weight, weight_scale, counts) if t is not None])
+    p = _lib.Product(R, E, N, K, _TYPES[out_dtype], 0, int(out is None), ldx, ldy)
+    _run(_lib.load().megamoe_int8_mm, what, device, _byref(p), x.data_ptr(), x_scale.data_ptr(), weight.data_ptr(),
+         weight_scale.data_ptr(), None if counts is None else counts.data_ptr(), y.data_ptr())
+    return y
+
+
+def int8_mm(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, *,
+            out_dtype: torch.dtype = torch.bfloat16, out: torch.Tensor | None = None) -> torch.Tensor:
+    """y [R, N] = (x @ weight^T) * x_scale[:, None] * weight_scale[None, :]: x int8 [R, K] with
+    fp32 scales [R], weight int8 [N, K] (out features by in features) with fp32 scales [N]. The
+    integer sums are exact; the result is bf16, fp16 or fp32."""
+    _device(x, "x")
+    if not isinstance(weight, torch.Tensor) or weight.dim() != 2:
+        raise ValueError("weight: expected int8 [out, in]")
+    return _int8(x, x_scale, weight, weight_scale, None, out_dtype, out, "int8_mm")
+
+
+def grouped_int8_mm(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor,
+                    counts: torch.Tensor, *, out_dtype: torch.dtype = torch.bfloat16,
+                    out: torch.Tensor | None = None) -> torch.Tensor:
+    """``int8_mm`` of every expert's rows with its own matrix: weight int8 [E, N, K] with fp32
+    scales [E, N], rows grouped by ``counts`` as in ``grouped_mm``."""
+    _device(x, "x")
+    if not isinstance(weight, torch.Tensor) or weight.dim() != 3:
+        raise ValueError("weight: expected int8 [experts, out, in]")
+    if not isinstance(counts, torch.Tensor):
+        raise ValueError("counts: expected int64 [experts]")
+    return _int8(x, x_scale, weight, weight_scale, counts, out_dtype, out, "grouped_int8_mm")
+
+
+def quantize_rows_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """int8 payload [R, C] and fp32 scales [R] of bf16, fp16 or fp32 rows: with a the row's
+    largest magnitude (at least 2^-100), scale = a / 127 and q = x * (127 / a) rounded to nearest
+    even. A row with NaN or an infinity gets the scale NaN and zeros."""
+    device = _device(x, "x")
+    if x.dtype not in _TYPES or x.dim() != 2:
+        raise ValueError("quantize_rows_int8 takes 2-D bfloat16, float16 or float32 rows")
+    x, ld = _rows(x, "x", x.dtype, None, device)
+    rows, cols = x.shape
+    q = torch.empty((rows, cols), dtype=torch.int8, device=device)
+    scale = torch.empty((rows,), dtype=torch.float32, device=device)
+    _run(_lib.load().megamoe_quantize_rows_int8, "quantize_rows_int8", device, rows, cols, ld, _TYPES[x.dtype],
+         x.data_ptr(), q.data_ptr(), scale.data_ptr())
+    return q, scale
