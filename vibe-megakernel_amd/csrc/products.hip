@@ -13,6 +13,7 @@
 
 #include <hip/hip_runtime.h>
 #include <atomic>
+#include <type_traits>
 #include <stddef.h>
 #include <stdint.h>
 
@@ -28,6 +29,16 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kMaxGroups = 1024;
 
+// One fragment of A by four of B, accumulated in place: left to itself, the compiler moves the
+// accumulators of a long loop between registers and spills. The wait states in front are those
+// between a VALU result and an MFMA that reads it, which it cannot see in here. (The results of
+// the last MFMAs may be read only after mfma_done().)
+#define MEGAMOE_MFMA4(name, c, a, b)                                                                             \
+  asm("s_nop 1\n\t" name " %0, %4, %5, %0\n\t" name " %1, %4, %6, %1\n\t" name " %2, %4, %7, %2\n\t" name        \
+      " %3, %4, %8, %3"                                                                                          \
+      : "+v"(c[0]), "+v"(c[1]), "+v"(c[2]), "+v"(c[3])                                                           \
+      : "v"(a), "v"(b[0]), "v"(b[1]), "v"(b[2]), "v"(b[3]))
+
 // What an element type of the operands brings: its accumulator and its 16x16 MFMA, whose lane l
 // holds row l % 16 and the 16 bytes at 16 * (l / 16) of both operands' c, and of the result rows
 // 4 * (l / 16) .. +3 (of A) in column l % 16 (of B).
@@ -39,6 +50,9 @@ struct Bf16 {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0,
                                                    0, 0);
   }
+  static __device__ __forceinline__ void mfma4(Acc (&c)[4], i32x4 a, const i32x4 (&b)[4]) {
+    MEGAMOE_MFMA4("v_mfma_f32_16x16x32_bf16", c, a, b);
+  }
 };
 struct Fp16 {
   using Elem = _Float16;
@@ -48,6 +62,9 @@ struct Fp16 {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0,
                                                   0);
   }
+  static __device__ __forceinline__ void mfma4(Acc (&c)[4], i32x4 a, const i32x4 (&b)[4]) {
+    MEGAMOE_MFMA4("v_mfma_f32_16x16x32_f16", c, a, b);
+  }
 };
 struct Int8 {
   using Elem = int8_t;
@@ -55,6 +72,9 @@ struct Int8 {
   static constexpr int kBytes = 1;
   static __device__ __forceinline__ Acc mfma(i32x4 a, i32x4 b, Acc c) {
     return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ void mfma4(Acc (&c)[4], i32x4 a, const i32x4 (&b)[4]) {
+    MEGAMOE_MFMA4("v_mfma_i32_16x16x64_i8", c, a, b);
   }
 };
 
@@ -321,30 +341,22 @@ __global__ __launch_bounds__(256) void k_wgrad_any(Args p) {
 // The tiled product (16-byte aligned operands)
 //
 // A persistent workgroup of eight wavefronts per CU computes tiles of 256 (i) by TJ (j) outputs,
-// stage by stage of 128 bytes of c. Each stage's operands are cut into four regions, the halves
-// A0, A1 (128 i each) and B0, B1 (TJ/2 j each), and a stage into four phases of one quadrant:
+// stage by stage of 128 bytes of c, each stage in two halves of 64 bytes. While one half's MFMAs
+// run from registers, the fragments of the next half are read from LDS: one operand's into
+// registers of its own, the other's in two parts of which the second takes the registers of
+// fragments that are done with. The second half of a stage is in registers before its first half
+// ends, so there the stage's buffer is free: one barrier a stage, at which no read is young,
+// and behind it the loads of the stage BUFFERS on, straight into LDS (64 KB or more in flight
+// per CU, no registers).
 //
-//   phase         0         1         2         3
-//   reads         A0        B1        A1        B0 of the next stage   (LDS -> registers)
-//   multiplies    A0 B0     A0 B1     A1 B1     A1 B0
-//   loads         B0        A0        B1        A1, of the stage after next, into the regions
-//                                               that the phase before freed
-//
-// A wavefront's share of a quadrant takes rows of both operands' halves, so that a region is
-// read by all wavefronts in one phase and free in the next. Every region is loaded seven phases
-// before it is read (about 100 KB in flight per CU, no registers), straight into LDS; the wait
-// in a phase lets the last six regions' loads stay pending. Wavefronts 4-7 run half a phase
-// behind 0-3 (one barrier more at the start), so on every SIMD one wavefront multiplies while the
-// other reads LDS and issues loads.
-//
-// The stages of consecutive tiles follow each other without a gap: loads run two stages ahead,
-// over the tile's end, so a tile's first stage is in LDS when the last tile's results are
-// stored. (A tile has at least two stages; a short c is padded with zeros.)
+// The stages of consecutive tiles follow each other without a gap: loads run over the tile's end,
+// so a tile's first stages are in LDS when the last tile's results are stored. (A tile has more
+// than BUFFERS stages; a short c is padded with zeros.)
 //
 // LDS layout. An operand with c contiguous: rows of 128 bytes, 16-byte chunk p of row r at
 // position p ^ (r % 8): one load instruction fills eight whole rows from full 128-byte lines,
 // and the MFMA's reads (16 rows of one chunk) fall into different banks. An operand with c
-// across: 64 rows (c) of 256 bytes (128 i or j), chunk p of row c at p ^ 2 f(c), f = c % 4 +
+// across: 64 rows (c) of 512 bytes (256 i or j), chunk p of row c at p ^ 2 f(c), f = c % 4 +
 // 4 (c / 8 % 2): the transposing reads (ds_read_b64_tr_b16: four c of 16 neighbours, for c = 8g ..
 // of the lane group g) fall into different banks as well.
 //
@@ -355,113 +367,90 @@ __global__ __launch_bounds__(256) void k_wgrad_any(Args p) {
 enum Form { kNT, kNN, kTN };  // y = x w^T, y = x w, dw = dy^T x
 
 constexpr int kThreads = 512, kTileI = 256, kStage = 128;
-constexpr int kRegionA = 128 * kStage;
 
 typedef int i32x2 __attribute__((ext_vector_type(2)));
 
+// Until this wavefront's LDS reads have arrived and at most N of its loads into LDS are pending;
+// then the workgroup's wavefronts meet. Nothing moves across it.
 template <int N>
-__device__ __forceinline__ void wait_loads() {
+__device__ __forceinline__ void meet() {
   static_assert(N >= 0 && N <= 63, "vmcnt holds 6 bits");
-  __builtin_amdgcn_s_waitcnt((N & 15) | (7 << 4) | (15 << 8) | (((N >> 4) & 3) << 14));
+  __builtin_amdgcn_sched_barrier(0);
+  // gfx9 s_waitcnt immediate: vmcnt[3:0] | expcnt[6:4] | lgkmcnt[11:8] | vmcnt[5:4] << 14
+  __builtin_amdgcn_s_waitcnt((N & 15) | (7 << 4) | (((N >> 4) & 3) << 14));
   asm volatile("" ::: "memory");
-}
-
-// A phase boundary: nothing moves across it.
-__device__ __forceinline__ void boundary() {
-  __builtin_amdgcn_sched_barrier(0);
   __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
   __builtin_amdgcn_sched_barrier(0);
 }
 
-// LDS reads in inline asm with their wait: the compiler would take an LDS read as depending on
-// every load into LDS in flight and wait for all of them.
-template <int OFF>
-__device__ __forceinline__ void read_rows(i32x4 (&f)[4][2], const uint32_t (&at)[2]) {
-  asm volatile(
-      "ds_read_b128 %0, %8 offset:%c10\n\tds_read_b128 %1, %9 offset:%c10\n\t"
-      "ds_read_b128 %2, %8 offset:%c11\n\tds_read_b128 %3, %9 offset:%c11\n\t"
-      "ds_read_b128 %4, %8 offset:%c12\n\tds_read_b128 %5, %9 offset:%c12\n\t"
-      "ds_read_b128 %6, %8 offset:%c13\n\tds_read_b128 %7, %9 offset:%c13\n\t"
-      "s_waitcnt lgkmcnt(0)"
-      : "=&v"(f[0][0]), "=&v"(f[0][1]), "=&v"(f[1][0]), "=&v"(f[1][1]), "=&v"(f[2][0]), "=&v"(f[2][1]),
-        "=&v"(f[3][0]), "=&v"(f[3][1])
-      : "v"(at[0]), "v"(at[1]), "i"(OFF), "i"(OFF + 2048), "i"(OFF + 4096), "i"(OFF + 6144)
-      : "memory");
-}
-template <int OFF>
-__device__ __forceinline__ void read_rows(i32x4 (&f)[2][2], const uint32_t (&at)[2]) {
-  asm volatile(
-      "ds_read_b128 %0, %4 offset:%c6\n\tds_read_b128 %1, %5 offset:%c6\n\t"
-      "ds_read_b128 %2, %4 offset:%c7\n\tds_read_b128 %3, %5 offset:%c7\n\t"
-      "s_waitcnt lgkmcnt(0)"
-      : "=&v"(f[0][0]), "=&v"(f[0][1]), "=&v"(f[1][0]), "=&v"(f[1][1])
-      : "v"(at[0]), "v"(at[1]), "i"(OFF), "i"(OFF + 2048)
-      : "memory");
-}
-// The transposing reads: per fragment and half stage (32 c) two, of c +0..3 and +4..7 of a lane.
-template <int OFF>
-__device__ __forceinline__ void read_cols2(i32x4 (&f)[2], i32x4 (&g)[2], uint32_t at_f, uint32_t at_g) {
-  i32x2 r[8];
-  asm volatile(
-      "ds_read_b64_tr_b16 %0, %8 offset:%c10\n\tds_read_b64_tr_b16 %1, %8 offset:%c11\n\t"
-      "ds_read_b64_tr_b16 %2, %8 offset:%c12\n\tds_read_b64_tr_b16 %3, %8 offset:%c13\n\t"
-      "ds_read_b64_tr_b16 %4, %9 offset:%c10\n\tds_read_b64_tr_b16 %5, %9 offset:%c11\n\t"
-      "ds_read_b64_tr_b16 %6, %9 offset:%c12\n\tds_read_b64_tr_b16 %7, %9 offset:%c13\n\t"
-      "s_waitcnt lgkmcnt(0)"
-      : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]), "=&v"(r[4]), "=&v"(r[5]), "=&v"(r[6]), "=&v"(r[7])
-      : "v"(at_f), "v"(at_g), "i"(OFF), "i"(OFF + 1024), "i"(OFF + 8192), "i"(OFF + 9216)
-      : "memory");
-  f[0] = __builtin_shufflevector(r[0], r[1], 0, 1, 2, 3);
-  f[1] = __builtin_shufflevector(r[2], r[3], 0, 1, 2, 3);
-  g[0] = __builtin_shufflevector(r[4], r[5], 0, 1, 2, 3);
-  g[1] = __builtin_shufflevector(r[6], r[7], 0, 1, 2, 3);
-}
-template <int OFF, int F>
-__device__ __forceinline__ void read_cols(i32x4 (&f)[F][2], const uint32_t (&at)[F]) {
-#pragma unroll
-  for (int i = 0; i < F; i += 2) read_cols2<OFF>(f[i], f[i + 1], at[i], at[i + 1]);
+// Wait states until the results of every MFMA issued so far can be read.
+__device__ __forceinline__ void mfma_done() {
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
 }
 
-// One operand as this wavefront loads and reads it. COL: c across (else contiguous). F: the
-// 16-row fragments of a wavefront in one half. L: load instructions of a wavefront per region.
-template <bool COL, int F, int L>
+// LDS at a byte address. The loads into LDS are inline asm without results (load_lds), so the
+// compiler counts the LDS reads alone and schedules them under the MFMAs by itself; the waits
+// for the loads are the phases' own.
+template <class T>
+__device__ __forceinline__ T lds_at(uint32_t at) {
+  return *(const __attribute__((address_space(3))) T*)(uintptr_t)at;
+}
+__device__ __forceinline__ i32x2 lds_transposed(uint32_t at) {
+  typedef short i16x4 __attribute__((ext_vector_type(4)));
+  return __builtin_bit_cast(
+      i32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(uintptr_t)at));
+}
+
+// One operand as this wavefront loads and reads it. COL: c across (else contiguous). L: the load
+// instructions of a wavefront per stage; load i fills the 1024 bytes wave + 8 i of the operand.
+template <bool COL, int L>
 struct Side {
-  uint32_t load[L];       // byte offset of the lane's 16 bytes from the half's first row, per instruction
-  uint32_t chunk;         // of them, the bytes along the contiguous dimension
-  uint32_t at[COL ? F : 2];  // LDS addresses of the lane's fragments in half 0, buffer `buf`
+  uint32_t load;   // byte offset of the lane's 16 bytes of the first load from the tile's first row
+  uint32_t next;   // from one load of the wavefront to the next
+  uint32_t chunk;  // of `load`, the bytes along the contiguous dimension
+  uint32_t at[COL ? 1 : 2];  // LDS addresses of the lane's part of fragment 0
 
-  // `first`: the wavefront's first row in a half; `base`: LDS address of half 0 of buffer 0.
+  // `first`: the wavefront's first row; `base`: LDS address of the operand in buffer 0.
   __device__ __forceinline__ void init(uint32_t ld, int wave, int first, uint32_t base) {
     const uint32_t lane = threadIdx.x & 63, g = lane >> 4;
     if constexpr (COL) {
-      chunk = ((lane & 15) ^ (2 * ((lane >> 4) | ((uint32_t)(wave & 1) << 2)))) * 16;
-#pragma unroll
-      for (int i = 0; i < L; ++i) load[i] = (4 * (L * wave + i) + (lane >> 4)) * ld + chunk;
-      const uint32_t f2 = 2 * (((lane >> 2) & 3) | ((g & 1) << 2));
-#pragma unroll
-      for (int f = 0; f < F; ++f)
-        at[f] = base + (8 * g + ((lane & 15) >> 2)) * 256 +
-                ((((uint32_t)(first >> 3) + 2 * f + ((lane & 3) >> 1)) ^ f2) << 4) + (lane & 1) * 8;
+      const uint32_t c = 2 * wave + (lane >> 5);
+      chunk = ((lane & 31) ^ (2 * ((c & 3) | ((c >> 1) & 4)))) * 16;
+      load = c * ld + chunk;
+      next = 16 * ld;
+      at[0] = base + (8 * g + ((lane & 15) >> 2)) * 512 +
+              ((((uint32_t)(first >> 3) + ((lane & 3) >> 1)) ^ (2 * (((lane >> 2) & 3) | ((g & 1) << 2)))) << 4) +
+              (lane & 1) * 8;
     } else {
       chunk = ((lane & 7) ^ (lane >> 3)) * 16;
-#pragma unroll
-      for (int i = 0; i < L; ++i) load[i] = (8 * (L * wave + i) + (lane >> 3)) * ld + chunk;
+      load = (8 * wave + (lane >> 3)) * ld + chunk;
+      next = 64 * ld;
 #pragma unroll
       for (int s = 0; s < 2; ++s)
         at[s] = base + ((uint32_t)first + (lane & 15)) * 128 + (((4 * s + g) ^ (lane & 7)) << 4);
     }
   }
-  // The reads to the other buffer, `by` bytes on (or back).
+  // The reads to another buffer, `by` bytes on (or back).
   __device__ __forceinline__ void move(uint32_t by) {
 #pragma unroll
     for (uint32_t& a : at) a += by;
   }
-  template <int OFF>
-  __device__ __forceinline__ void read(i32x4 (&f)[F][2]) const {
-    if constexpr (COL)
-      read_cols<OFF>(f, at);
-    else
-      read_rows<OFF>(f, at);
+  // Fragments BEGIN .. BEGIN + N - 1 (16 rows each) of the stage's half s.
+  template <int BEGIN, int N>
+  __device__ __forceinline__ void read(i32x4 (&f)[N], int s) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if constexpr (COL) {
+        const uint32_t p = (at[0] ^ (32u * (BEGIN + i))) + 16384u * s;
+        const i32x2 lo = lds_transposed(p), hi = lds_transposed(p + 2048);
+        f[i] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3);
+      } else {
+        f[i] = lds_at<i32x4>(at[s] + 2048 * (BEGIN + i));
+      }
+    }
   }
 };
 
@@ -478,21 +467,36 @@ __device__ __forceinline__ T uniform(T v) {
   }
 }
 
-// 16 bytes a lane into LDS (1024 consecutive ones from `lds`), from `base` + at + along; zero from
-// `bytes` on.
-__device__ __forceinline__ void load_lds(uint8_t* lds, const uint8_t* base, uint32_t bytes, uint32_t at, uint32_t along) {
+// 16 bytes a lane into LDS (1024 consecutive ones from byte address `to`), from `base` + at +
+// along; zero from `bytes` on.
+__device__ __forceinline__ void load_lds(uint32_t to, const uint8_t* base, uint32_t bytes, uint32_t at, uint32_t along) {
 #ifdef __HIP_DEVICE_COMPILE__
-  const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)uniform(base), 0, uniform(bytes), 0x00020000);
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)lds, 16, at, along, 0, 0);
+  const uint64_t b = (uint64_t)uniform(base);
+  const i32x4 rsrc = {(int)(uint32_t)b, (int)((uint32_t)(b >> 32) & 0xffffu), (int)uniform(bytes), 0x00020000};
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+               :
+               : "s"(uniform(to)), "v"(at), "s"(rsrc), "s"(uniform(along))
+               : "memory", "m0");
 #endif
 }
 
-// One region's loads: `live` tells the lanes whose bytes exist, `bytes` the length of the rows that do.
-template <int L>
-__device__ __forceinline__ void load_region(uint8_t* lds, int wave, const uint8_t* base, uint32_t bytes,
-                                            const uint32_t (&at)[L], bool live, uint32_t along) {
+// Loads BEGIN .. END-1 of one operand's stage: `live` tells the lanes whose bytes exist, `bytes` the
+// length of the rows that do (the range check takes the sum of both offsets).
+template <int BEGIN, int END, class S>
+__device__ __forceinline__ void load_stage(uint32_t to, int wave, const uint8_t* base, uint32_t bytes, const S& side,
+                                           bool live, uint32_t along) {
+  const uint32_t at = live ? side.load : kOutside;
 #pragma unroll
-  for (int i = 0; i < L; ++i) load_lds(lds + (L * wave + i) * 1024, base, bytes, live ? at[i] : kOutside, along);
+  for (int i = BEGIN; i < END; ++i)
+    load_lds(to + (uint32_t)(wave + 8 * i) * 1024, base, bytes, at, along + i * side.next);
+}
+
+// The lane index, opaque to the compiler: what is derived from it is not kept in registers across
+// the loop that it is used behind.
+__device__ __forceinline__ int opaque_lane() {
+  int lane = threadIdx.x & 63;
+  asm volatile("" : "+v"(lane));
+  return lane;
 }
 
 // The groups' tables in LDS: rows and row tiles before each group (entry g), to the end of the
@@ -529,23 +533,14 @@ __device__ bool make_table(Table& t, const Args& p, int height) {
   return t.rows[kMaxGroups] <= (uint32_t)p.rows;
 }
 
-__device__ __forceinline__ uint32_t lds_word(const uint32_t* p) {
-  uint32_t v;
-  asm volatile("ds_read_b32 %0, %1\n\ts_waitcnt lgkmcnt(0)"
-               : "=&v"(v)
-               : "v"((uint32_t)(uintptr_t)(__attribute__((address_space(3))) const uint32_t*)p)
-               : "memory");
-  return v;
-}
-
 // Row tile `tile` (below the table's total): its group and rows.
 __device__ __forceinline__ Tile table_tile(const Table& t, int tile, int height) {
   const int lane = threadIdx.x & 63;
-  const uint32_t coarse = lds_word(&t.tiles[16 * lane + 16]);
+  const uint32_t coarse = t.tiles[16 * lane + 16];
   const int block = __builtin_popcountll(__ballot(coarse <= (uint32_t)tile));
-  const uint32_t fine = lds_word(&t.tiles[16 * block + 1 + (lane & 15)]);
+  const uint32_t fine = t.tiles[16 * block + 1 + (lane & 15)];
   const int group = 16 * block + __builtin_popcountll(__ballot(fine <= (uint32_t)tile) & 0xffff);
-  const uint32_t v = lds_word(lane == 0 ? &t.tiles[group] : &t.rows[group + (lane & 1 ? 0 : 1)]);
+  const uint32_t v = lane == 0 ? t.tiles[group] : t.rows[group + (lane & 1 ? 0 : 1)];
   const int first = (int)lane_value(v, 1) + (tile - (int)lane_value(v, 0)) * height;
   return Tile{group, first, min(first + height, (int)lane_value(v, 2))};
 }
@@ -564,23 +559,26 @@ constexpr int kBand = 4;  // row tiles that are walked together, column by colum
 
 // What the loads need of a tile, and the results.
 struct Work {
-  const uint8_t* a;  // first row of A's half 0
+  const uint8_t* a;  // first rows of the operands
   const uint8_t* b;
   int group, first, last;  // rows of y (the products), of the group (the weights' gradient)
   int i0, j0;              // first column and row of the output tile (j0: within rows first..last)
   int stages;
+  uint32_t rows_a, rows_b;  // bytes of the rows that exist (c contiguous)
 };
 
 template <class Ty, class Out, Form FORM, int TJ>
 __global__ __launch_bounds__(kThreads, 2) void k_tiles(Args p) {
   constexpr bool kAcol = FORM != kNT, kBcol = FORM == kTN;
-  constexpr int WI = TJ == 256 ? 2 : 4, WJ = 8 / WI;     // wavefronts along i and j
-  constexpr int FA = 128 / WI / 16, FB = TJ / 2 / WJ / 16;  // fragments of a wavefront in a half
-  constexpr int LA = 2, LB = TJ / 128;                    // loads of a wavefront per region
-  constexpr int kRegionB = TJ / 2 * kStage;
-  constexpr int kPending = 3 * (LA + LB);
+  constexpr int WI = TJ == 256 ? 2 : 4, WJ = 8 / WI;              // wavefronts along i and j
+  constexpr int FA = kTileI / WI / 16, FB = TJ / WJ / 16, FH = FA / 2;  // fragments of a wavefront
+  static_assert(FB == 4, "mfma4");
+  constexpr int LA = kTileI / 64, LB = TJ / 64;                   // loads of a wavefront per stage
+  constexpr int BUFFERS = TJ == 256 ? 2 : 3;
+  constexpr int kBytesA = kTileI * kStage, kBytes = kBytesA + TJ * kStage;
+  constexpr int kPending = (BUFFERS - 2) * (LA + LB);
   constexpr int kC = kStage / Ty::kBytes;  // c of one stage
-  __shared__ __align__(1024) uint8_t lds[4 * kRegionA + 4 * kRegionB];
+  __shared__ __align__(1024) uint8_t lds[BUFFERS * kBytes];
   __shared__ Table table;
 
   const int wave = uniform((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -616,12 +614,12 @@ __global__ __launch_bounds__(kThreads, 2) void k_tiles(Args p) {
       const int tiles_j = (p.n + TJ - 1) / TJ;
       w.group = rt / tiles_j;
       w.j0 = rt % tiles_j * TJ;
-      const uint32_t v = lds_word(&table.rows[w.group + (lane & 1)]);
+      const uint32_t v = table.rows[w.group + (lane & 1)];
       w.first = (int)lane_value(v, 0);
       w.last = (int)lane_value(v, 1);
       w.a = p.x + (int64_t)w.first * lda + (int64_t)w.i0 * Ty::kBytes;
       w.b = p.w + (int64_t)w.first * ldb + (int64_t)w.j0 * Ty::kBytes;
-      w.stages = max(2, (w.last - w.first + kC - 1) / kC);
+      w.stages = max(BUFFERS + 1, (w.last - w.first + kC - 1) / kC);
     } else {
       const Tile t = table_tile(table, rt, TJ);
       w.group = t.group;
@@ -631,8 +629,10 @@ __global__ __launch_bounds__(kThreads, 2) void k_tiles(Args p) {
       w.a = p.w + (size_t)w.group * p.n * p.k * Ty::kBytes +
             (FORM == kNT ? (int64_t)w.i0 * lda : (int64_t)w.i0 * Ty::kBytes);
       w.b = p.x + (int64_t)w.first * ldb;
-      w.stages = max(2, (p.k + kC - 1) / kC);
+      w.stages = max(BUFFERS + 1, (p.k + kC - 1) / kC);
     }
+    w.rows_a = uniform((uint32_t)min(p.n - w.i0, kTileI) * (uint32_t)lda);
+    w.rows_b = uniform((uint32_t)(w.last - w.first) * (uint32_t)ldb);
     return w;
   };
 
@@ -644,172 +644,151 @@ __global__ __launch_bounds__(kThreads, 2) void k_tiles(Args p) {
   int stage = 0;                   // of `ahead`
   bool more = true;
 
-  Side<kAcol, FA, LA> sa;
-  Side<kBcol, FB, LB> sb;
+  Side<kAcol, LA> sa;
+  Side<kBcol, LB> sb;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
-  sa.init((uint32_t)lda, wave, wi * (128 / WI), lds0);
-  sb.init((uint32_t)ldb, wave, wj * (TJ / 2 / WJ), lds0 + 4 * kRegionA);
+  sa.init((uint32_t)lda, wave, wi * (kTileI / WI), lds0);
+  sb.init((uint32_t)ldb, wave, wj * (TJ / WJ), lds0 + kBytesA);
 
-  // Loads of half `h` of A (or B) at the load cursor into buffer `buf`.
-  auto load_a = [&](int h, int buf) {
-    uint8_t* const to = lds + (2 * buf + h) * kRegionA;
+  // Part `part` (of two) of the loads at the load cursor, into buffer `buf`.
+  auto load_a = [&](auto part, int buf) {
+    constexpr int B = part.value * LA / 2, E = B + LA / 2;
+    const uint32_t to = lds0 + buf * kBytes;
     if constexpr (kAcol) {
       const int rows = (FORM == kTN ? ahead.last - ahead.first : p.k) - stage * kC;
-      const bool live = sa.chunk + 256u * h < (uint32_t)(ni - ahead.i0) * Ty::kBytes;
-      load_region(to, wave, ahead.a + (int64_t)stage * kC * lda + 256 * h,
-                  more ? (uint32_t)min(max(rows, 0), kC) * (uint32_t)lda : 0u, sa.load, live, 0u);
+      load_stage<B, E>(to, wave, ahead.a + (int64_t)stage * kC * lda,
+                       more ? (uint32_t)min(max(rows, 0), kC) * (uint32_t)lda : 0u, sa,
+                       sa.chunk < (uint32_t)(ni - ahead.i0) * Ty::kBytes, 0u);
     } else {
-      const int rows = min(max(p.n - ahead.i0 - 128 * h, 0), 128);
-      load_region(to, wave, ahead.a + (int64_t)128 * h * lda, more ? (uint32_t)rows * (uint32_t)lda : 0u, sa.load,
-                  (uint32_t)stage * kStage + sa.chunk < (uint32_t)p.k * Ty::kBytes, (uint32_t)stage * kStage);
+      load_stage<B, E>(to, wave, ahead.a, ahead.rows_a, sa,
+                       (uint32_t)stage * kStage + sa.chunk < (uint32_t)p.k * Ty::kBytes, (uint32_t)stage * kStage);
     }
   };
-  auto load_b = [&](int h, int buf) {
-    uint8_t* const to = lds + 4 * kRegionA + (2 * buf + h) * kRegionB;
+  auto load_b = [&](auto part, int buf) {
+    constexpr int B = part.value * LB / 2, E = B + LB / 2;
+    const uint32_t to = lds0 + buf * kBytes + kBytesA;
     if constexpr (kBcol) {
       const int rows = ahead.last - ahead.first - stage * kC;
-      const bool live = sb.chunk + 256u * h < (uint32_t)(p.n - ahead.j0) * Ty::kBytes;
-      load_region(to, wave, ahead.b + (int64_t)stage * kC * ldb + 256 * h,
-                  more ? (uint32_t)min(max(rows, 0), kC) * (uint32_t)ldb : 0u, sb.load, live, 0u);
+      load_stage<B, E>(to, wave, ahead.b + (int64_t)stage * kC * ldb,
+                       more ? (uint32_t)min(max(rows, 0), kC) * (uint32_t)ldb : 0u, sb,
+                       sb.chunk < (uint32_t)(p.n - ahead.j0) * Ty::kBytes, 0u);
     } else {
-      const int rows = min(max(ahead.last - ahead.first - TJ / 2 * h, 0), TJ / 2);
-      load_region(to, wave, ahead.b + (int64_t)(TJ / 2) * h * ldb, more ? (uint32_t)rows * (uint32_t)ldb : 0u, sb.load,
-                  (uint32_t)stage * kStage + sb.chunk < (uint32_t)p.k * Ty::kBytes, (uint32_t)stage * kStage);
+      load_stage<B, E>(to, wave, ahead.b, ahead.rows_b, sb,
+                       (uint32_t)stage * kStage + sb.chunk < (uint32_t)p.k * Ty::kBytes, (uint32_t)stage * kStage);
     }
   };
+  constexpr std::integral_constant<int, 0> kFirst{};
+  constexpr std::integral_constant<int, 1> kSecond{};
   // The load cursor to the next stage, over the tile's end.
   auto advance = [&]() {
     if (++stage < ahead.stages || !more) return;
     stage = 0;
     tile = xcd_tile(++step, total);
     more = tile >= 0;
-    if (more) ahead = locate_work(tile);
+    if (more)
+      ahead = locate_work(tile);
+    else
+      ahead.rows_a = ahead.rows_b = 0;
   };
 
-  typename Ty::Acc acc[2][2][FA][FB];
-  i32x4 a[FA][2], b0[FB][2], b1[FB][2], bn[FB][2];
+  typename Ty::Acc acc[FA][FB];
+  // A's fragments of the lower and upper rows, one set more, and B's of two halves.
+  i32x4 x[FH], y[FH], z[FH], b0[FB], b1[FB];
   auto clear = [&]() {
 #pragma unroll
-    for (int h = 0; h < 4; ++h)
+    for (int f = 0; f < FA; ++f)
 #pragma unroll
-      for (int f = 0; f < FA; ++f)
-#pragma unroll
-        for (int t = 0; t < FB; ++t) acc[h >> 1][h & 1][f][t] = typename Ty::Acc{0, 0, 0, 0};
+      for (int t = 0; t < FB; ++t) acc[f][t] = typename Ty::Acc{0, 0, 0, 0};
   };
-  auto multiply = [&](typename Ty::Acc(&c)[FA][FB], const i32x4(&b)[FB][2]) {
-    __builtin_amdgcn_s_setprio(1);
+  // A fragments f0 .. f0 + n - 1 (of the tile) from a[at ..]; the scheduler keeps it in one piece.
+  auto multiply = [&](const i32x4(&a)[FH], int f0, const i32x4(&b)[FB], int at, int n) {
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int s = 0; s < 2; ++s)
-#pragma unroll
-      for (int f = 0; f < FA; ++f)
-#pragma unroll
-        for (int t = 0; t < FB; ++t) c[f][t] = Ty::mfma(a[f][s], b[t][s], c[f][t]);
-    __builtin_amdgcn_s_setprio(0);
+    for (int f = at; f < at + n; ++f) Ty::mfma4(acc[f0 + f], a[f], b);
+    __builtin_amdgcn_sched_barrier(0);
   };
   // Results: lane l has i = 4 (l / 16) .. +3 of a fragment at j = l % 16.
   auto store = [&]() {
+    mfma_done();
+    const int lane = opaque_lane();
     const bool wide = ldo % 4 == 0 && (uintptr_t)p.out % (4 * sizeof(Out)) == 0;
     const int nj = FORM == kTN ? p.n : now.last - now.first;
     Out* const base = FORM == kTN ? out + (size_t)now.group * p.n * p.k : out + (int64_t)now.first * ldo;
 #pragma unroll
-    for (int hb = 0; hb < 2; ++hb)
+    for (int t = 0; t < FB; ++t) {
+      const int j = now.j0 + wj * (TJ / WJ) + 16 * t + (lane & 15);
+      if (j >= nj) continue;
+      Out* const row = base + (int64_t)j * ldo;
+      float sx = 0.f;
+      if constexpr (Ty::kBytes == 1) sx = p.sx[now.first + j];
 #pragma unroll
-      for (int t = 0; t < FB; ++t) {
-        const int j = now.j0 + TJ / 2 * hb + wj * (TJ / 2 / WJ) + 16 * t + (lane & 15);
-        if (j >= nj) continue;
-        Out* const row = base + (int64_t)j * ldo;
-        float sx = 0.f;
-        if constexpr (Ty::kBytes == 1) sx = p.sx[now.first + j];
+      for (int f = 0; f < FA; ++f) {
+        const int i = now.i0 + wi * (kTileI / WI) + 16 * f + 4 * (lane >> 4);
+        typedef Out Out4 __attribute__((ext_vector_type(4)));
+        Out4 v;
 #pragma unroll
-        for (int ha = 0; ha < 2; ++ha)
+        for (int e = 0; e < 4; ++e) {
+          if constexpr (Ty::kBytes == 1)
+            v[e] = (Out)scaled(acc[f][t][e], sx, i + e < ni ? p.sw[(size_t)now.group * p.n + i + e] : 0.f);
+          else
+            v[e] = (Out)acc[f][t][e];
+        }
+        if (wide && i + 3 < ni) {
+          *reinterpret_cast<Out4*>(row + i) = v;
+        } else {
 #pragma unroll
-          for (int f = 0; f < FA; ++f) {
-            const int i = now.i0 + 128 * ha + wi * (128 / WI) + 16 * f + 4 * (lane >> 4);
-            typedef Out Out4 __attribute__((ext_vector_type(4)));
-            Out4 v;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              if constexpr (Ty::kBytes == 1)
-                v[e] = (Out)scaled(acc[ha][hb][f][t][e], sx,
-                                   i + e < ni ? p.sw[(size_t)now.group * p.n + i + e] : 0.f);
-              else
-                v[e] = (Out)acc[ha][hb][f][t][e];
-            }
-            if (wide && i + 3 < ni) {
-              *reinterpret_cast<Out4*>(row + i) = v;
-            } else {
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (i + e < ni) row[i + e] = v[e];
-            }
-          }
+          for (int e = 0; e < 4; ++e)
+            if (i + e < ni) row[i + e] = v[e];
+        }
       }
+    }
   };
 
-  load_b(0, 0);
-  load_a(0, 0);
-  load_b(1, 0);
-  load_a(1, 0);
-  advance();
-  load_b(0, 1);
-  load_a(0, 1);
-  load_b(1, 1);
-  load_a(1, 1);
-  advance();
-  wait_loads<kPending>();
-  boundary();
-  sb.template read<0>(b0);
-  boundary();
-  if (wave >= 4) boundary();
-  clear();
-  int left = now.stages, buf = 0;
-  for (;;) {
-    load_b(0, buf);
-    sa.template read<0>(a);
-    wait_loads<kPending>();
-    boundary();
-    multiply(acc[0][0], b0);
-    boundary();
-
-    load_a(0, buf);
-    sb.template read<kRegionB>(b1);
-    wait_loads<kPending>();
-    boundary();
-    multiply(acc[0][1], b1);
-    boundary();
-
-    load_b(1, buf);
-    sa.template read<kRegionA>(a);
-    wait_loads<kPending>();
-    boundary();
-    multiply(acc[1][1], b1);
-    boundary();
-
-    load_a(1, buf);
-    sa.move(buf ? -2 * kRegionA : 2 * kRegionA);
-    sb.move(buf ? -2 * kRegionB : 2 * kRegionB);
-    sb.template read<0>(bn);
-    wait_loads<kPending>();
-    boundary();
-    multiply(acc[1][0], b0);
-    boundary();
-#pragma unroll
-    for (int t = 0; t < FB; ++t) {
-      b0[t][0] = bn[t][0];
-      b0[t][1] = bn[t][1];
-    }
-    buf ^= 1;
-    if (--left == 0) {
-      store();
-      if (!more) break;  // (the loads are two stages ahead: past the last tile only now)
-      now = ahead;
-      left = now.stages;
-      clear();
-    }
+  for (int i = 0; i < BUFFERS; ++i) {
+    load_a(kFirst, i);
+    load_a(kSecond, i);
+    load_b(kFirst, i);
+    load_b(kSecond, i);
     advance();
   }
-  if (wave < 4) boundary();
-  wait_loads<0>();  // loads into LDS may not outlive the workgroup
+  meet<(BUFFERS - 1) * (LA + LB)>();
+  sb.template read<0>(b0, 0);
+  sa.template read<0>(x, 0);
+  sa.template read<FH>(y, 0);
+  int buf = 0;
+  for (;;) {
+    clear();
+    for (int left = now.stages; left > 0; --left) {
+      // First half of the stage: x, y and b0. The second half's fragments arrive in z, x and b1.
+      sb.template read<0>(b1, 1);
+      sa.template read<0>(z, 1);
+      multiply(x, 0, b0, 0, FH);
+      sa.template read<FH>(x, 1);
+      multiply(y, FH, b0, 0, FH);
+      meet<kPending>();
+      // Second half: z, x and b1. The next stage's first half arrives in x, y and b0.
+      const int to = buf;
+      buf = buf + 1 == BUFFERS ? 0 : buf + 1;
+      sa.move(buf == 0 ? -(BUFFERS - 1) * kBytes : kBytes);
+      sb.move(buf == 0 ? -(BUFFERS - 1) * kBytes : kBytes);
+      sb.template read<0>(b0, 0);
+      sa.template read<FH>(y, 0);
+      load_a(kFirst, to);
+      multiply(x, FH, b1, 0, FH / 2);
+      load_a(kSecond, to);
+      multiply(x, FH, b1, FH / 2, FH / 2);
+      sa.template read<0>(x, 0);
+      load_b(kFirst, to);
+      multiply(z, 0, b1, 0, FH / 2);
+      load_b(kSecond, to);
+      multiply(z, 0, b1, FH / 2, FH / 2);
+      advance();
+    }
+    store();
+    if (!more) break;  // (the loads are BUFFERS + 1 stages ahead, within the next tile)
+    now = ahead;
+  }
+  __builtin_amdgcn_s_waitcnt(0);  // loads into LDS may not outlive the workgroup
 }
 
 // ---------------------------------------------------------------------------------------
