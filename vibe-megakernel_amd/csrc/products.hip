@@ -13,6 +13,7 @@
 
 #include <hip/hip_runtime.h>
 #include <atomic>
+#include <math.h>
 #include <type_traits>
 #include <stddef.h>
 #include <stdint.h>
@@ -134,23 +135,29 @@ __device__ Tile locate(const int64_t* counts, int groups, int rows, int height, 
   uint32_t row0 = 0, tile0 = 0;
   bool bad = false;
   Tile found{kNoTile, 0, 0};
-  for (int g0 = 0; g0 < groups; g0 += 64) {
-    int64_t c = g0 + lane < groups ? counts[g0 + lane] : 0;
-    const bool wrong = c < 0 || c > rows;
-    bad |= __ballot(wrong) != 0;
-    const uint32_t n = wrong ? 0 : (uint32_t)c, t = (n + (uint32_t)height - 1) / (uint32_t)height;
-    const uint32_t rows_to = add_sat(row0, wave_scan(n)), tiles_to = add_sat(tile0, wave_scan(t));
-    const uint64_t mask = __ballot((uint32_t)tile < tiles_to && (uint32_t)tile >= tiles_to - t);
-    if (mask) {
-      const int l = __builtin_ctzll(mask);
-      const int start = (int)(lane_value(rows_to, l) - lane_value(n, l));
-      const int within = tile - (int)(lane_value(tiles_to, l) - lane_value(t, l));
-      found.group = g0 + l;
-      found.first = start + within * height;
-      found.last = min(found.first + height, (int)lane_value(rows_to, l));
+  for (int g0 = 0; g0 < groups; g0 += 256) {
+    int64_t c[4];  // four loads in flight
+#pragma unroll
+    for (int q = 0; q < 4; ++q) c[q] = g0 + 64 * q + lane < groups ? counts[g0 + 64 * q + lane] : 0;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      if (g0 + 64 * q >= groups) break;
+      const bool wrong = c[q] < 0 || c[q] > rows;
+      bad |= __ballot(wrong) != 0;
+      const uint32_t n = wrong ? 0 : (uint32_t)c[q], t = (n + (uint32_t)height - 1) / (uint32_t)height;
+      const uint32_t rows_to = add_sat(row0, wave_scan(n)), tiles_to = add_sat(tile0, wave_scan(t));
+      const uint64_t mask = __ballot((uint32_t)tile < tiles_to && (uint32_t)tile >= tiles_to - t);
+      if (mask) {
+        const int l = __builtin_ctzll(mask);
+        const int start = (int)(lane_value(rows_to, l) - lane_value(n, l));
+        const int within = tile - (int)(lane_value(tiles_to, l) - lane_value(t, l));
+        found.group = g0 + 64 * q + l;
+        found.first = start + within * height;
+        found.last = min(found.first + height, (int)lane_value(rows_to, l));
+      }
+      row0 = lane_value(rows_to, 63);
+      tile0 = lane_value(tiles_to, 63);
     }
-    row0 = lane_value(rows_to, 63);
-    tile0 = lane_value(tiles_to, 63);
   }
   if (bad || row0 > (uint32_t)rows) {
     const int64_t first = (int64_t)tile * height;
@@ -356,7 +363,7 @@ __global__ __launch_bounds__(256) void k_wgrad_any(Args p) {
 // LDS layout. An operand with c contiguous: rows of 128 bytes, 16-byte chunk p of row r at
 // position p ^ (r % 8): one load instruction fills eight whole rows from full 128-byte lines,
 // and the MFMA's reads (16 rows of one chunk) fall into different banks. An operand with c
-// across: 64 rows (c) of 512 bytes (256 i or j), chunk p of row c at p ^ 2 f(c), f = c % 4 +
+// across: 64 rows (c) of all the tile's i or j, chunk p of row c at p ^ 2 f(c), f = c % 4 +
 // 4 (c / 8 % 2): the transposing reads (ds_read_b64_tr_b16: four c of 16 neighbours, for c = 8g ..
 // of the lane group g) fall into different banks as well.
 //
@@ -366,7 +373,7 @@ __global__ __launch_bounds__(256) void k_wgrad_any(Args p) {
 
 enum Form { kNT, kNN, kTN };  // y = x w^T, y = x w, dw = dy^T x
 
-constexpr int kThreads = 512, kTileI = 256, kStage = 128;
+constexpr int kThreads = 512, kStage = 128;
 
 typedef int i32x2 __attribute__((ext_vector_type(2)));
 
@@ -408,6 +415,7 @@ __device__ __forceinline__ i32x2 lds_transposed(uint32_t at) {
 // instructions of a wavefront per stage; load i fills the 1024 bytes wave + 8 i of the operand.
 template <bool COL, int L>
 struct Side {
+  static constexpr uint32_t kRow = COL ? 128 * L : 128;  // bytes of a row in LDS (COL: all 64 L columns)
   uint32_t load;   // byte offset of the lane's 16 bytes of the first load from the tile's first row
   uint32_t next;   // from one load of the wavefront to the next
   uint32_t chunk;  // of `load`, the bytes along the contiguous dimension
@@ -417,11 +425,12 @@ struct Side {
   __device__ __forceinline__ void init(uint32_t ld, int wave, int first, uint32_t base) {
     const uint32_t lane = threadIdx.x & 63, g = lane >> 4;
     if constexpr (COL) {
-      const uint32_t c = 2 * wave + (lane >> 5);
-      chunk = ((lane & 31) ^ (2 * ((c & 3) | ((c >> 1) & 4)))) * 16;
+      constexpr uint32_t kRows = 1024 / kRow, kLanes = 64 / kRows;  // of one load, of one row
+      const uint32_t c = kRows * wave + lane / kLanes;
+      chunk = ((lane % kLanes) ^ (2 * ((c & 3) | ((c >> 1) & 4)))) * 16;
       load = c * ld + chunk;
-      next = 16 * ld;
-      at[0] = base + (8 * g + ((lane & 15) >> 2)) * 512 +
+      next = 8 * kRows * ld;
+      at[0] = base + (8 * g + ((lane & 15) >> 2)) * kRow +
               ((((uint32_t)(first >> 3) + ((lane & 3) >> 1)) ^ (2 * (((lane >> 2) & 3) | ((g & 1) << 2)))) << 4) +
               (lane & 1) * 8;
     } else {
@@ -444,8 +453,8 @@ struct Side {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       if constexpr (COL) {
-        const uint32_t p = (at[0] ^ (32u * (BEGIN + i))) + 16384u * s;
-        const i32x2 lo = lds_transposed(p), hi = lds_transposed(p + 2048);
+        const uint32_t p = (at[0] ^ (32u * (BEGIN + i))) + 32 * kRow * s;
+        const i32x2 lo = lds_transposed(p), hi = lds_transposed(p + 4 * kRow);
         f[i] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3);
       } else {
         f[i] = lds_at<i32x4>(at[s] + 2048 * (BEGIN + i));
@@ -469,26 +478,39 @@ __device__ __forceinline__ T uniform(T v) {
 
 // 16 bytes a lane into LDS (1024 consecutive ones from byte address `to`), from `base` + at +
 // along; zero from `bytes` on.
+template <bool ONCE>
 __device__ __forceinline__ void load_lds(uint32_t to, const uint8_t* base, uint32_t bytes, uint32_t at, uint32_t along) {
 #ifdef __HIP_DEVICE_COMPILE__
   const uint64_t b = (uint64_t)uniform(base);
   const i32x4 rsrc = {(int)(uint32_t)b, (int)((uint32_t)(b >> 32) & 0xffffu), (int)uniform(bytes), 0x00020000};
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
-               :
-               : "s"(uniform(to)), "v"(at), "s"(rsrc), "s"(uniform(along))
-               : "memory", "m0");
+  if constexpr (ONCE)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen nt lds"
+                 :
+                 : "s"(uniform(to)), "v"(at), "s"(rsrc), "s"(uniform(along))
+                 : "memory", "m0");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+                 :
+                 : "s"(uniform(to)), "v"(at), "s"(rsrc), "s"(uniform(along))
+                 : "memory", "m0");
 #endif
 }
 
-// Loads BEGIN .. END-1 of one operand's stage: `live` tells the lanes whose bytes exist, `bytes` the
-// length of the rows that do (the range check takes the sum of both offsets).
-template <int BEGIN, int END, class S>
-__device__ __forceinline__ void load_stage(uint32_t to, int wave, const uint8_t* base, uint32_t bytes, const S& side,
-                                           bool live, uint32_t along) {
-  const uint32_t at = live ? side.load : kOutside;
-#pragma unroll
-  for (int i = BEGIN; i < END; ++i)
-    load_lds(to + (uint32_t)(wave + 8 * i) * 1024, base, bytes, at, along + i * side.next);
+// Load I of one operand's stage: `live` tells the lanes whose bytes exist, `bytes` the length of
+// the rows that do (the range check takes the sum of both offsets).
+template <int I, bool ONCE = false, class S>
+__device__ __forceinline__ void load_one(uint32_t to, int wave, const uint8_t* base, uint32_t bytes, const S& side,
+                                         bool live, uint32_t along) {
+  load_lds<ONCE>(to + (uint32_t)(wave + 8 * I) * 1024, base, bytes, live ? side.load : kOutside, along + I * side.next);
+}
+
+// Calls f(std::integral_constant<int, I>{}) for I = B .. E-1.
+template <int B, int E, class F>
+__device__ __forceinline__ void static_for(F&& f) {
+  if constexpr (B < E) {
+    f(std::integral_constant<int, B>{});
+    static_for<B + 1, E>(f);
+  }
 }
 
 // The lane index, opaque to the compiler: what is derived from it is not kept in registers across
@@ -499,10 +521,11 @@ __device__ __forceinline__ int opaque_lane() {
   return lane;
 }
 
-// The groups' tables in LDS: rows and row tiles before each group (entry g), to the end of the
-// last (entry `groups` and on).
+// The groups' tables in LDS: before each group (entry g), and to the end of the last (entry `groups`
+// and on), its rows, its tiles of more than half the height (all but its last, perhaps) and its
+// smaller ones (its last, perhaps).
 struct Table {
-  uint32_t rows[kMaxGroups + 16], tiles[kMaxGroups + 16];
+  uint32_t rows[kMaxGroups + 16], tiles[kMaxGroups + 16], small[kMaxGroups + 16];
 };
 
 // Fills the table; false if the counts do not fit the rows. Every thread of the workgroup calls it.
@@ -514,46 +537,65 @@ __device__ bool make_table(Table& t, const Args& p, int height) {
   }
   __syncthreads();
   if (threadIdx.x < 64) {
-    uint32_t row0 = 0, tile0 = 0;
+    uint32_t row0 = 0, tile0 = 0, small0 = 0;
     for (int g0 = 0; g0 < p.groups; g0 += 64) {
-      const uint32_t c = g0 + lane < p.groups ? t.rows[g0 + lane] : 0u;
-      const uint32_t n = (uint32_t)(((uint64_t)c + height - 1) / (uint32_t)height);
+      const uint32_t c = g0 + lane < p.groups ? t.rows[g0 + lane] : 0u, rest = c % (uint32_t)height;
+      const uint32_t half = (uint32_t)height / 2, n = c / (uint32_t)height + (rest > half), s = rest > 0 && rest <= half;
       const uint32_t rows_to = add_sat(row0, wave_scan(c)), tiles_to = add_sat(tile0, wave_scan(n));
+      const uint32_t small_to = small0 + wave_scan(s);
       t.rows[g0 + lane] = rows_to - c;  // exact wherever the sums are
       t.tiles[g0 + lane] = tiles_to - n;
+      t.small[g0 + lane] = small_to - s;
       row0 = lane_value(rows_to, 63);
       tile0 = lane_value(tiles_to, 63);
+      small0 = lane_value(small_to, 63);
     }
     for (int g = (p.groups + 63) / 64 * 64 + lane; g < kMaxGroups + 16; g += 64) {
       t.rows[g] = row0;
       t.tiles[g] = tile0;
+      t.small[g] = small0;
     }
   }
   __syncthreads();
   return t.rows[kMaxGroups] <= (uint32_t)p.rows;
 }
 
-// Row tile `tile` (below the table's total): its group and rows.
+// Row tile `tile` (below the table's total): its group and rows. The tiles of more than half the
+// height come first, so that the last ones of a launch are the short ones.
 __device__ __forceinline__ Tile table_tile(const Table& t, int tile, int height) {
   const int lane = threadIdx.x & 63;
-  const uint32_t coarse = t.tiles[16 * lane + 16];
-  const int block = __builtin_popcountll(__ballot(coarse <= (uint32_t)tile));
-  const uint32_t fine = t.tiles[16 * block + 1 + (lane & 15)];
-  const int group = 16 * block + __builtin_popcountll(__ballot(fine <= (uint32_t)tile) & 0xffff);
-  const uint32_t v = lane == 0 ? t.tiles[group] : t.rows[group + (lane & 1 ? 0 : 1)];
-  const int first = (int)lane_value(v, 1) + (tile - (int)lane_value(v, 0)) * height;
-  return Tile{group, first, min(first + height, (int)lane_value(v, 2))};
+  const int big = uniform((int)t.tiles[kMaxGroups]);
+  const bool small = tile >= big;
+  const uint32_t* const before = small ? t.small : t.tiles;
+  const uint32_t at = (uint32_t)(small ? tile - big : tile);
+  const int block = __builtin_popcountll(__ballot(before[16 * lane + 16] <= at));
+  const int group = 16 * block + __builtin_popcountll(__ballot(before[16 * block + 1 + (lane & 15)] <= at) & 0xffff);
+  const uint32_t v = lane < 2 ? t.tiles[group + lane] : t.rows[group + (lane & 1)];
+  const int within = small ? (int)(lane_value(v, 1) - lane_value(v, 0)) : (int)(at - lane_value(v, 0));
+  const int first = (int)lane_value(v, 2) + within * height;
+  return Tile{group, first, min(first + height, (int)lane_value(v, 3))};
 }
 
 // Workgroups of a grid go to the eight XCDs in turn, each with an L2 of its own: step s of the
-// persistent grid is `grid` consecutive tiles, of which each XCD takes a consecutive eighth. -1:
-// none for this workgroup.
+// persistent grid is `grid` consecutive tiles, of which each XCD takes a consecutive eighth. The
+// last tiles of several steps go to the workgroups whose step before was the shortest, the last
+// ones. -1: none for this workgroup.
 __device__ __forceinline__ int xcd_tile(int step, int total) {
   const int grid = (int)gridDim.x, first = step * grid, left = min(total - first, grid);
   if (left <= 0) return -1;
-  const int each = (left + 7) / 8, at = ((int)blockIdx.x & 7) * each + ((int)blockIdx.x >> 3);
-  return ((int)blockIdx.x >> 3) < each && at < left ? first + at : -1;
+  const int xcd = (int)blockIdx.x & 7, in = (int)blockIdx.x >> 3;
+  if (step > 0 && left < grid) {
+    const int at = xcd * (grid / 8) + in - (grid - left);
+    return at >= 0 ? first + at : -1;
+  }
+  const int each = (left + 7) / 8, at = xcd * each + in;
+  return in < each && at < left ? first + at : -1;
 }
+
+// Groups start at different places of c: rows whose pitch is a large power of two (4 KB and on) would
+// otherwise have all workgroups at addresses of few memory channels (256 experts of 2 rows, 4096 by
+// 2048: 655 us without, 607 with it; pitches of no such power are indifferent to it).
+constexpr uint32_t kTurn = 3;
 
 constexpr int kBand = 4;  // row tiles that are walked together, column by column
 
@@ -564,18 +606,19 @@ struct Work {
   int group, first, last;  // rows of y (the products), of the group (the weights' gradient)
   int i0, j0;              // first column and row of the output tile (j0: within rows first..last)
   int stages;
+  int turn;                // the stage that comes first (c is walked in a circle)
   uint32_t rows_a, rows_b;  // bytes of the rows that exist (c contiguous)
 };
 
-template <class Ty, class Out, Form FORM, int TJ>
+template <class Ty, class Out, Form FORM, int TI, int TJ, bool ONCE>
 __global__ __launch_bounds__(kThreads, 2) void k_tiles(Args p) {
   constexpr bool kAcol = FORM != kNT, kBcol = FORM == kTN;
-  constexpr int WI = TJ == 256 ? 2 : 4, WJ = 8 / WI;              // wavefronts along i and j
-  constexpr int FA = kTileI / WI / 16, FB = TJ / WJ / 16, FH = FA / 2;  // fragments of a wavefront
+  constexpr int WJ = TJ / 64, WI = 8 / WJ;                        // wavefronts along i and j
+  constexpr int FA = TI / WI / 16, FB = TJ / WJ / 16, FH = FA / 2;  // fragments of a wavefront
   static_assert(FB == 4, "mfma4");
-  constexpr int LA = kTileI / 64, LB = TJ / 64;                   // loads of a wavefront per stage
-  constexpr int BUFFERS = TJ == 256 ? 2 : 3;
-  constexpr int kBytesA = kTileI * kStage, kBytes = kBytesA + TJ * kStage;
+  constexpr int LA = TI / 64, LB = TJ / 64;                   // loads of a wavefront per stage
+  constexpr int kBytesA = TI * kStage, kBytes = kBytesA + TJ * kStage;
+  constexpr int BUFFERS = (147456 / kBytes);
   constexpr int kPending = (BUFFERS - 2) * (LA + LB);
   constexpr int kC = kStage / Ty::kBytes;  // c of one stage
   __shared__ __align__(1024) uint8_t lds[BUFFERS * kBytes];
@@ -586,7 +629,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_tiles(Args p) {
   Out* const out = reinterpret_cast<Out*>(p.out);
   const int ni = FORM == kTN ? p.k : p.n;
   const int64_t ldo = FORM == kTN ? p.k : p.ldy;
-  const int tiles_i = (ni + kTileI - 1) / kTileI;
+  const int tiles_i = (ni + TI - 1) / TI;
 
   const bool fits = uniform((int)make_table(table, p, TJ)) != 0;
   if (!fits) {  // NaN everywhere
@@ -596,7 +639,8 @@ __global__ __launch_bounds__(kThreads, 2) void k_tiles(Args p) {
     return;
   }
   const int used = uniform((int)table.rows[kMaxGroups]);
-  const int row_tiles = FORM == kTN ? p.groups * ((p.n + TJ - 1) / TJ) : uniform((int)table.tiles[kMaxGroups]);
+  const int row_tiles = FORM == kTN ? p.groups * ((p.n + TJ - 1) / TJ)
+                                    : uniform((int)(table.tiles[kMaxGroups] + table.small[kMaxGroups]));
   const int total = row_tiles * tiles_i;
   if (FORM != kTN && p.fill_rest)
     for (int64_t r = used + blockIdx.x; r < p.rows; r += gridDim.x)
@@ -609,7 +653,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_tiles(Args p) {
     const int high = min(kBand, row_tiles - band * kBand);
     const int rt = band * kBand + in % high, it = in / high;
     Work w;
-    w.i0 = it * kTileI;
+    w.i0 = it * TI;
     if constexpr (FORM == kTN) {
       const int tiles_j = (p.n + TJ - 1) / TJ;
       w.group = rt / tiles_j;
@@ -631,7 +675,8 @@ __global__ __launch_bounds__(kThreads, 2) void k_tiles(Args p) {
       w.b = p.x + (int64_t)w.first * ldb;
       w.stages = max(BUFFERS + 1, (p.k + kC - 1) / kC);
     }
-    w.rows_a = uniform((uint32_t)min(p.n - w.i0, kTileI) * (uint32_t)lda);
+    w.turn = FORM == kTN ? 0 : uniform((int)((uint32_t)w.group * kTurn % (uint32_t)w.stages));
+    w.rows_a = uniform((uint32_t)min(p.n - w.i0, TI) * (uint32_t)lda);
     w.rows_b = uniform((uint32_t)(w.last - w.first) * (uint32_t)ldb);
     return w;
   };
@@ -647,38 +692,40 @@ __global__ __launch_bounds__(kThreads, 2) void k_tiles(Args p) {
   Side<kAcol, LA> sa;
   Side<kBcol, LB> sb;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
-  sa.init((uint32_t)lda, wave, wi * (kTileI / WI), lds0);
+  sa.init((uint32_t)lda, wave, wi * (TI / WI), lds0);
   sb.init((uint32_t)ldb, wave, wj * (TJ / WJ), lds0 + kBytesA);
 
-  // Part `part` (of two) of the loads at the load cursor, into buffer `buf`.
-  auto load_a = [&](auto part, int buf) {
-    constexpr int B = part.value * LA / 2, E = B + LA / 2;
+  // Load `i` of A's (or B's) loads at the load cursor, into buffer `buf`.
+  auto at_stage = [&]() {
+    const int s = stage + ahead.turn;
+    return s >= ahead.stages && more ? s - ahead.stages : s;
+  };
+  auto load_a = [&](auto i, int buf) {
+    const int stage = at_stage();
     const uint32_t to = lds0 + buf * kBytes;
     if constexpr (kAcol) {
       const int rows = (FORM == kTN ? ahead.last - ahead.first : p.k) - stage * kC;
-      load_stage<B, E>(to, wave, ahead.a + (int64_t)stage * kC * lda,
+      load_one<i.value, ONCE>(to, wave, ahead.a + (int64_t)stage * kC * lda,
                        more ? (uint32_t)min(max(rows, 0), kC) * (uint32_t)lda : 0u, sa,
                        sa.chunk < (uint32_t)(ni - ahead.i0) * Ty::kBytes, 0u);
     } else {
-      load_stage<B, E>(to, wave, ahead.a, ahead.rows_a, sa,
+      load_one<i.value, ONCE>(to, wave, ahead.a, ahead.rows_a, sa,
                        (uint32_t)stage * kStage + sa.chunk < (uint32_t)p.k * Ty::kBytes, (uint32_t)stage * kStage);
     }
   };
-  auto load_b = [&](auto part, int buf) {
-    constexpr int B = part.value * LB / 2, E = B + LB / 2;
+  auto load_b = [&](auto i, int buf) {
+    const int stage = at_stage();
     const uint32_t to = lds0 + buf * kBytes + kBytesA;
     if constexpr (kBcol) {
       const int rows = ahead.last - ahead.first - stage * kC;
-      load_stage<B, E>(to, wave, ahead.b + (int64_t)stage * kC * ldb,
+      load_one<i.value>(to, wave, ahead.b + (int64_t)stage * kC * ldb,
                        more ? (uint32_t)min(max(rows, 0), kC) * (uint32_t)ldb : 0u, sb,
                        sb.chunk < (uint32_t)(p.n - ahead.j0) * Ty::kBytes, 0u);
     } else {
-      load_stage<B, E>(to, wave, ahead.b, ahead.rows_b, sb,
+      load_one<i.value>(to, wave, ahead.b, ahead.rows_b, sb,
                        (uint32_t)stage * kStage + sb.chunk < (uint32_t)p.k * Ty::kBytes, (uint32_t)stage * kStage);
     }
   };
-  constexpr std::integral_constant<int, 0> kFirst{};
-  constexpr std::integral_constant<int, 1> kSecond{};
   // The load cursor to the next stage, over the tile's end.
   auto advance = [&]() {
     if (++stage < ahead.stages || !more) return;
@@ -700,89 +747,125 @@ __global__ __launch_bounds__(kThreads, 2) void k_tiles(Args p) {
 #pragma unroll
       for (int t = 0; t < FB; ++t) acc[f][t] = typename Ty::Acc{0, 0, 0, 0};
   };
-  // A fragments f0 .. f0 + n - 1 (of the tile) from a[at ..]; the scheduler keeps it in one piece.
+  // Fragments at .. at + n - 1 of a[], which are f0 .. of the tile, by b; the scheduler keeps it in
+  // one piece.
   auto multiply = [&](const i32x4(&a)[FH], int f0, const i32x4(&b)[FB], int at, int n) {
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int f = at; f < at + n; ++f) Ty::mfma4(acc[f0 + f], a[f], b);
     __builtin_amdgcn_sched_barrier(0);
   };
+
   // Results: lane l has i = 4 (l / 16) .. +3 of a fragment at j = l % 16.
   auto store = [&]() {
     mfma_done();
     const int lane = opaque_lane();
-    const bool wide = ldo % 4 == 0 && (uintptr_t)p.out % (4 * sizeof(Out)) == 0;
+    constexpr int kWide = 16 / (int)sizeof(Out);  // outputs of one store
+    typedef Out OutN __attribute__((ext_vector_type(kWide)));
+    const bool wide = ldo % kWide == 0 && (uintptr_t)p.out % 16 == 0;
     const int nj = FORM == kTN ? p.n : now.last - now.first;
     Out* const base = FORM == kTN ? out + (size_t)now.group * p.n * p.k : out + (int64_t)now.first * ldo;
 #pragma unroll
     for (int t = 0; t < FB; ++t) {
       const int j = now.j0 + wj * (TJ / WJ) + 16 * t + (lane & 15);
-      if (j >= nj) continue;
-      Out* const row = base + (int64_t)j * ldo;
       float sx = 0.f;
-      if constexpr (Ty::kBytes == 1) sx = p.sx[now.first + j];
-#pragma unroll
-      for (int f = 0; f < FA; ++f) {
-        const int i = now.i0 + wi * (kTileI / WI) + 16 * f + 4 * (lane >> 4);
-        typedef Out Out4 __attribute__((ext_vector_type(4)));
-        Out4 v;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if constexpr (Ty::kBytes == 1)
-            v[e] = (Out)scaled(acc[f][t][e], sx, i + e < ni ? p.sw[(size_t)now.group * p.n + i + e] : 0.f);
-          else
-            v[e] = (Out)acc[f][t][e];
+      if constexpr (Ty::kBytes == 1) sx = j < nj ? p.sx[now.first + j] : 0.f;
+      auto value = [&](int f, int e) {
+        if constexpr (Ty::kBytes == 1) {
+          const int i = now.i0 + wi * (TI / WI) + 16 * f + 4 * (lane >> 4) + e;
+          return scaled(acc[f][t][e], sx, i < ni ? p.sw[(size_t)now.group * p.n + i] : 0.f);
+        } else {
+          return acc[f][t][e];
         }
-        if (wide && i + 3 < ni) {
-          *reinterpret_cast<Out4*>(row + i) = v;
+      };
+      auto put = [&](int i, OutN v) {
+        if (j >= nj) return;
+        Out* const row = base + (int64_t)j * ldo;
+        if (wide && i + kWide <= ni) {
+          *reinterpret_cast<OutN*>(row + i) = v;
         } else {
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
+          for (int e = 0; e < kWide; ++e)
             if (i + e < ni) row[i + e] = v[e];
+        }
+      };
+#pragma unroll
+      for (int f = 0; f < FA; f += kWide / 4) {
+        const int i = now.i0 + wi * (TI / WI) + 16 * f;
+        if constexpr (kWide == 4) {
+          put(i + 4 * (lane >> 4), OutN{(Out)value(f, 0), (Out)value(f, 1), (Out)value(f, 2), (Out)value(f, 3)});
+        } else {
+          // Two fragments' halves change places between neighbouring groups of 16 lanes, so that a
+          // lane has eight neighbours of one of them.
+          typedef Out Out2 __attribute__((ext_vector_type(2)));
+          uint32_t u[2][2];
+#pragma unroll
+          for (int q = 0; q < 2; ++q)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              u[q][h] = __builtin_bit_cast(uint32_t, Out2{(Out)value(f + q, 2 * h), (Out)value(f + q, 2 * h + 1)});
+          const auto lo = __builtin_amdgcn_permlane16_swap(u[0][0], u[1][0], false, false);
+          const auto hi = __builtin_amdgcn_permlane16_swap(u[0][1], u[1][1], false, false);
+          const i32x4 all = {(int)lo[0], (int)hi[0], (int)lo[1], (int)hi[1]};
+          put(i + 16 * ((lane >> 4) & 1) + 8 * (lane >> 5), __builtin_bit_cast(OutN, all));
         }
       }
     }
   };
 
   for (int i = 0; i < BUFFERS; ++i) {
-    load_a(kFirst, i);
-    load_a(kSecond, i);
-    load_b(kFirst, i);
-    load_b(kSecond, i);
+    static_for<0, LA>([&](auto l) { load_a(l, i); });
+    static_for<0, LB>([&](auto l) { load_b(l, i); });
     advance();
   }
   meet<(BUFFERS - 1) * (LA + LB)>();
   sb.template read<0>(b0, 0);
   sa.template read<0>(x, 0);
   sa.template read<FH>(y, 0);
-  int buf = 0;
+  int buf = 0, last = 0;  // the buffer that is read, and the one before it
+  auto next_buffer = [&]() {
+    last = buf;
+    buf = buf + 1 == BUFFERS ? 0 : buf + 1;
+    sa.move(buf == 0 ? -(BUFFERS - 1) * kBytes : kBytes);
+    sb.move(buf == 0 ? -(BUFFERS - 1) * kBytes : kBytes);
+  };
   for (;;) {
     clear();
-    for (int left = now.stages; left > 0; --left) {
-      // First half of the stage: x, y and b0. The second half's fragments arrive in z, x and b1.
-      sb.template read<0>(b1, 1);
-      sa.template read<0>(z, 1);
-      multiply(x, 0, b0, 0, FH);
-      sa.template read<FH>(x, 1);
-      multiply(y, FH, b0, 0, FH);
-      meet<kPending>();
-      // Second half: z, x and b1. The next stage's first half arrives in x, y and b0.
-      const int to = buf;
-      buf = buf + 1 == BUFFERS ? 0 : buf + 1;
-      sa.move(buf == 0 ? -(BUFFERS - 1) * kBytes : kBytes);
-      sb.move(buf == 0 ? -(BUFFERS - 1) * kBytes : kBytes);
+    const int nj = FORM == kTN ? p.n - now.j0 : now.last - now.first;
+    if (wj * (TJ / WJ) < nj) {
+      for (int left = now.stages; left > 0; --left) {
+        // First half of the stage: x, y and b0. The second half's fragments arrive in z, x and b1.
+        sb.template read<0>(b1, 1);
+        sa.template read<0>(z, 1);
+        multiply(x, 0, b0, 0, FH);
+        sa.template read<FH>(x, 1);
+        multiply(y, FH, b0, 0, FH);
+        meet<kPending>();
+        // Second half: z, x and b1. The next stage's first half arrives in x, y and b0.
+        next_buffer();
+        sb.template read<0>(b0, 0);
+        static_for<0, LA>([&](auto l) { load_a(l, last); });
+        sa.template read<FH>(y, 0);
+        multiply(x, FH, b1, 0, FH / 2);
+        static_for<0, LB>([&](auto l) { load_b(l, last); });
+        multiply(x, FH, b1, FH / 2, FH - FH / 2);
+        sa.template read<0>(x, 0);
+        multiply(z, 0, b1, 0, FH);
+        advance();
+      }
+    } else {
+      // No rows for this wavefront: it loads, and leaves the MFMAs to the one beside it (of a tile
+      // of at most half the height, every SIMD has one of either kind).
+      for (int left = now.stages; left > 0; --left) {
+        meet<kPending>();
+        next_buffer();
+        static_for<0, LA>([&](auto l) { load_a(l, last); });
+        static_for<0, LB>([&](auto l) { load_b(l, last); });
+        advance();
+      }
       sb.template read<0>(b0, 0);
-      sa.template read<FH>(y, 0);
-      load_a(kFirst, to);
-      multiply(x, FH, b1, 0, FH / 2);
-      load_a(kSecond, to);
-      multiply(x, FH, b1, FH / 2, FH / 2);
       sa.template read<0>(x, 0);
-      load_b(kFirst, to);
-      multiply(z, 0, b1, 0, FH / 2);
-      load_b(kSecond, to);
-      multiply(z, 0, b1, FH / 2, FH / 2);
-      advance();
+      sa.template read<FH>(y, 0);
     }
     store();
     if (!more) break;  // (the loads are BUFFERS + 1 stages ahead, within the next tile)
@@ -792,35 +875,185 @@ __global__ __launch_bounds__(kThreads, 2) void k_tiles(Args p) {
 }
 
 // ---------------------------------------------------------------------------------------
-// Rows to int8
+// The product by strips (16-byte aligned operands, c contiguous): calls with too few tiles to
+// occupy the GPU
+//
+// A workgroup of eight wavefronts computes 16 MI by 16 MJ outputs, the wavefronts taking the
+// 128-byte steps of c in turn; their sums are added through LDS in wavefront order. A step's
+// fragments are loaded straight into registers: lane l has the 32 bytes at 32 * (l / 16) of row
+// l % 16, so four lanes cover a whole 128-byte line (the MFMAs see c in another order, the same
+// for both operands). kDeep steps are in flight per wavefront, 16 wavefronts on a CU.
 // ---------------------------------------------------------------------------------------
 
-template <class In>
+constexpr int kDeep = 4;
+
+// 16 bytes a lane from `base` + at + along; zero from `bytes` on.
+__device__ __forceinline__ i32x4 load_16(const uint8_t* base, uint32_t bytes, uint32_t at, uint32_t along) {
+#ifdef __HIP_DEVICE_COMPILE__
+  const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)uniform(base), 0, uniform(bytes), 0x00020000);
+  return __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(r, at, along, 0));
+#else
+  return i32x4{};
+#endif
+}
+
+template <class Ty, class Out, int MI, int MJ>
+__global__ __launch_bounds__(kThreads, 4) void k_strips(Args p) {
+  __shared__ typename Ty::Acc part[8][MI * MJ][64];
+  const int wave = uniform((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const uint32_t kbytes = (uint32_t)p.k * Ty::kBytes;
+  const uint32_t lda = kbytes, ldb = (uint32_t)(p.ldx * Ty::kBytes);
+  const int steps = (int)((kbytes + 127) / 128);
+  Out* const out = reinterpret_cast<Out*>(p.out);
+  const int64_t total = (int64_t)p.tiles_j * p.tiles_i;
+  for (int64_t at = blockIdx.x; at < total; at += gridDim.x) {
+    const int i0 = (int)(at % p.tiles_i) * 16 * MI, i1 = min(i0 + 16 * MI, p.n);
+    const Tile t = locate(p.counts, p.groups, p.rows, 16 * MJ, (int)(at / p.tiles_i));
+    if (t.group == kNoTile) continue;
+    if (t.group < 0) {
+      if (t.group == kBad || p.fill_rest)
+        fill_rows(out, p.ldy, t.first, t.last, i0, i1, t.group == kBad ? __builtin_nanf("") : 0.f);
+      continue;
+    }
+    const uint8_t* const a = p.w + ((size_t)t.group * p.n + i0) * kbytes;
+    const uint8_t* const b = p.x + (int64_t)t.first * p.ldx * Ty::kBytes;
+    const uint32_t rows_a = (uint32_t)(i1 - i0) * lda, rows_b = (uint32_t)(t.last - t.first) * ldb;
+    const uint32_t part_c = (uint32_t)(lane >> 4) * 32;
+    typename Ty::Acc acc[MI][MJ] = {};
+    for (int s0 = wave; s0 < steps; s0 += 8 * kDeep) {
+      i32x4 fa[kDeep][MI][2], fb[kDeep][MJ][2];
+#pragma unroll
+      for (int d = 0; d < kDeep; ++d) {
+        const uint32_t along = (uint32_t)(s0 + 8 * d) * 128;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t c = part_c + 16 * h;
+          const bool live = along + c < kbytes;
+#pragma unroll
+          for (int m = 0; m < MI; ++m)
+            fa[d][m][h] = load_16(a, rows_a, live ? (16 * m + (lane & 15)) * lda + c : kOutside, along);
+#pragma unroll
+          for (int m = 0; m < MJ; ++m)
+            fb[d][m][h] = load_16(b, rows_b, live ? (16 * m + (lane & 15)) * ldb + c : kOutside, along);
+        }
+      }
+#pragma unroll
+      for (int d = 0; d < kDeep; ++d)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int m = 0; m < MI; ++m)
+#pragma unroll
+            for (int n = 0; n < MJ; ++n) acc[m][n] = Ty::mfma(fa[d][m][h], fb[d][n][h], acc[m][n]);
+    }
+#pragma unroll
+    for (int m = 0; m < MI; ++m)
+#pragma unroll
+      for (int n = 0; n < MJ; ++n) part[wave][m * MJ + n][lane] = acc[m][n];
+    __syncthreads();
+    for (int o = threadIdx.x; o < 256 * MI * MJ; o += kThreads) {
+      const int j = o / (16 * MI), i = o % (16 * MI);
+      if (i0 + i < i1 && t.first + j < t.last) {
+        const int f = i / 16 * MJ + j / 16, l = (i % 16 / 4) * 16 + j % 16;
+        auto sum = part[0][f][l][i % 4];
+#pragma unroll
+        for (int w = 1; w < 8; ++w) sum += part[w][f][l][i % 4];
+        float v;
+        if constexpr (Ty::kBytes == 1)
+          v = scaled(sum, p.sx[t.first + j], p.sw[(size_t)t.group * p.n + i0 + i]);
+        else
+          v = sum;
+        out[(int64_t)(t.first + j) * p.ldy + i0 + i] = (Out)v;
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// ---------------------------------------------------------------------------------------
+// Rows to int8
+//
+// One pass over the row: it is held in registers (CHUNKS 16-byte chunks a thread) between the
+// search for the largest magnitude and the rounding, so each byte is read once. The search runs
+// on the magnitudes' bits, where NaN and infinity are the largest. Rows of other alignments, and
+// longer ones, are read twice, element by element.
+// ---------------------------------------------------------------------------------------
+
+// The row's scale (thread 0 writes it) and 127 / a from the largest magnitude's bits; 0 for a row
+// that holds NaN or an infinity.
+__device__ __forceinline__ float int8_factor(uint32_t largest, float* scale, bool write) {
+  const bool finite = largest < 0x7f800000u;
+  const float a = fmaxf(__uint_as_float(largest), 0x1p-100f);
+  if (write) *scale = finite ? a / 127.0f : __builtin_nanf("");
+  return finite ? 127.0f / a : 0.f;
+}
+
+// x * factor rounded to nearest even; 0 for factor 0 (whatever x is).
+__device__ __forceinline__ int to_int8(float x, float factor) {
+  return factor == 0.f ? 0 : (int)__builtin_rintf(x * factor);
+}
+
+__device__ __forceinline__ uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+
+// The largest of the workgroup's (or, ROW_WAVE, of the wavefront's) values.
+template <bool ROW_WAVE>
+__device__ __forceinline__ uint32_t largest_of(uint32_t v, uint32_t* part) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) v = max(v, (uint32_t)__shfl_xor((int)v, d, 64));
+  if constexpr (!ROW_WAVE) {
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = max(max(part[0], part[1]), max(part[2], part[3]));
+  }
+  return v;
+}
+
+// A row for each wavefront (ROW_WAVE) or for each workgroup of 256 threads; rows of 16-byte
+// chunks, at most CHUNKS a thread.
+template <class In, int CHUNKS, bool ROW_WAVE>
 __global__ __launch_bounds__(256) void k_quantize_int8(int64_t rows, int cols, int64_t ldx, const In* x, int8_t* q,
                                                        float* scale) {
-  __shared__ float part[4];
+  constexpr int kPer = 16 / (int)sizeof(In), kWidth = ROW_WAVE ? 64 : 256;
+  typedef In Chunk __attribute__((ext_vector_type(kPer)));
+  __shared__ uint32_t part[4];
+  const int64_t row = ROW_WAVE ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
+  if (row >= rows) return;
+  const int t = ROW_WAVE ? threadIdx.x & 63 : threadIdx.x;
+  const Chunk* const from = reinterpret_cast<const Chunk*>(x + row * ldx);
+  const int chunks = cols / kPer;
+  Chunk v[CHUNKS];
+#pragma unroll
+  for (int i = 0; i < CHUNKS; ++i) v[i] = t + i * kWidth < chunks ? from[t + i * kWidth] : Chunk{};
+  uint32_t largest = 0;
+#pragma unroll
+  for (int i = 0; i < CHUNKS; ++i)
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) largest = max(largest, magnitude((float)v[i][e]));
+  largest = largest_of<ROW_WAVE>(largest, part);
+  const float factor = int8_factor(largest, scale + row, t == 0);
+#pragma unroll
+  for (int i = 0; i < CHUNKS; ++i) {
+    if (t + i * kWidth >= chunks) break;
+    typedef int8_t Bytes __attribute__((ext_vector_type(kPer)));
+    Bytes b;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) b[e] = (int8_t)to_int8((float)v[i][e], factor);
+    reinterpret_cast<Bytes*>(q + row * cols)[t + i * kWidth] = b;
+  }
+}
+
+template <class In>
+__global__ __launch_bounds__(256) void k_quantize_int8_any(int64_t rows, int cols, int64_t ldx, const In* x, int8_t* q,
+                                                           float* scale) {
+  __shared__ uint32_t part[4];
   for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
     const In* const row = x + r * ldx;
-    float a = 0.f;
-    bool odd = false;
-    for (int c = threadIdx.x; c < cols; c += 256) {
-      const float v = __builtin_fabsf((float)row[c]);
-      odd |= !(v < __builtin_inff());
-      a = fmaxf(a, v);
-    }
-    if (odd) a = __builtin_inff();
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) a = fmaxf(a, __shfl_xor(a, d, 64));
-    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = a;
+    uint32_t largest = 0;
+    for (int c = threadIdx.x; c < cols; c += 256) largest = max(largest, magnitude((float)row[c]));
+    largest = largest_of<false>(largest, part);
+    const float factor = int8_factor(largest, scale + r, threadIdx.x == 0);
+    for (int c = threadIdx.x; c < cols; c += 256) q[r * cols + c] = (int8_t)to_int8((float)row[c], factor);
     __syncthreads();
-    a = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
-    __syncthreads();
-    const bool finite = a < __builtin_inff();
-    a = fmaxf(a, 0x1p-100f);
-    const float inv = 127.0f / a;
-    if (threadIdx.x == 0) scale[r] = finite ? a / 127.0f : __builtin_nanf("");
-    for (int c = threadIdx.x; c < cols; c += 256)
-      q[r * cols + c] = finite ? (int8_t)(int)__builtin_rintf((float)row[c] * inv) : (int8_t)0;
   }
 }
 
@@ -828,7 +1061,7 @@ __global__ __launch_bounds__(256) void k_quantize_int8(int64_t rows, int cols, i
 // Host
 // ---------------------------------------------------------------------------------------
 
-constexpr int64_t kMaxStrideBytes = 8 << 20, kMaxBlocks = 1 << 20;
+constexpr int64_t kMaxStrideBytes = 8 << 20, kMaxBlocks = 1 << 20, kMaxRowBlocks = 1 << 23;  // (a grid holds fewer than 2^32 threads)
 
 int launched() { return hipGetLastError() == hipSuccess ? MEGAMOE_OK : MEGAMOE_ERR_HIP; }
 
@@ -860,6 +1093,16 @@ int launch_any(Args a, hipStream_t stream) {
   return launched();
 }
 
+template <class Ty, class Out, int MI, int MJ>
+int launch_strips(Args a, hipStream_t stream) {
+  a.tiles_j = (int)row_tiles(a.rows, a.groups, 16 * MJ, a.counts != nullptr);
+  a.tiles_i = (int)ceil_div(a.n, 16 * MI);
+  const int64_t total = (int64_t)a.tiles_j * a.tiles_i;
+  hipLaunchKernelGGL((k_strips<Ty, Out, MI, MJ>), dim3((unsigned)(total < kMaxBlocks ? total : kMaxBlocks)),
+                     dim3(kThreads), 0, stream, a);
+  return launched();
+}
+
 template <class Ty>
 int launch_wgrad_any(Args a, hipStream_t stream) {
   a.tiles_j = (int)ceil_div(a.n, kAnyTile);
@@ -883,15 +1126,15 @@ int compute_units() {
   return n;
 }
 
-template <class Ty, class Out, Form FORM, int TJ>
+template <class Ty, class Out, Form FORM, int TI, int TJ, bool ONCE>
 int launch_tiles(Args a, hipStream_t stream) {
   const int cus = compute_units();
   if (cus <= 0) return MEGAMOE_ERR_HIP;
   const int64_t rows = FORM == kTN ? a.groups * ceil_div(a.n, TJ) : row_tiles(a.rows, a.groups, TJ, a.counts != nullptr);
-  const int64_t total = rows * ceil_div(FORM == kTN ? a.k : a.n, kTileI);
+  const int64_t total = rows * ceil_div(FORM == kTN ? a.k : a.n, TI);
   if (total > INT32_MAX) return MEGAMOE_ERR_UNSUPPORTED;
   const int64_t grid = ceil_div(total < cus ? total : cus, 8) * 8;
-  hipLaunchKernelGGL((k_tiles<Ty, Out, FORM, TJ>), dim3((unsigned)grid), dim3(kThreads), 0, stream, a);
+  hipLaunchKernelGGL((k_tiles<Ty, Out, FORM, TI, TJ, ONCE>), dim3((unsigned)grid), dim3(kThreads), 0, stream, a);
   return launched();
 }
 
@@ -918,10 +1161,98 @@ bool chunks(const void* p, int64_t ld, int64_t width, int elem) {
   return aligned(p, 16) && ld * elem % 16 == 0 && width * elem % 16 == 0;
 }
 
+// What is known of a call before it runs: the groups that have rows, and rows of one of those.
+// Groups' counts are on the device, so as many as uniform routing would hit.
+struct Load {
+  double groups, rows;
+};
+
+Load expected(const Args& a) {
+  if (!a.counts) return Load{1.0, (double)a.rows};
+  const double mean = (double)a.rows / a.groups, hit = a.groups * (1.0 - exp(-mean));
+  return Load{hit, a.rows / hit};
+}
+
+// Row tiles of `height` to expect: one of a group of up to half the height, half a tile more than
+// full ones of larger groups.
+double expected_tiles(const Args& a, const Load& l, int height) {
+  if (!a.counts) return (double)ceil_div(a.rows, height);
+  return l.groups * (l.rows <= height / 2 ? 1.0 : l.rows / height + 0.5);
+}
+
+double clamp01(double v) { return v < 0 ? 0 : v > 1 ? 1 : v; }
+
+// The tiled kernel for a product. Each size's time is its rounds of the GPU (not a whole number of
+// them costs about a third of one) times a tile's: its stages, and what its start and end cost in
+// stages. A stage of 256x128 takes 0.585 of one of 256x256 where the MFMAs decide (8192 cubed in
+// bf16: 204 us a round against 120) and 0.78 where the weights stream from memory (rows of a group
+// up to 128); one of 128x128 0.585 and 0.5 of 256x128's (7168 by 2048, 2 rows a group: 131 us a
+// round against 66).
+//
+// ONCE loads the weights past the caches: they are not read again where a group's rows make up to
+// two tiles (225 of 256 experts hit, 7168 by 2048 in bf16: 1078 us without, 955 with it; 1024 rows a
+// group and more lose up to 7% by it).
 template <class Ty, class Out, Form FORM>
 int launch_rows(const Args& a, hipStream_t s) {
-  return a.rows >= (int64_t)192 * a.groups ? launch_tiles<Ty, Out, FORM, 256>(a, s)
-                                           : launch_tiles<Ty, Out, FORM, 128>(a, s);
+  const int cus = compute_units();
+  if (cus <= 0) return MEGAMOE_ERR_HIP;
+  const Load l = expected(a);
+  const double kbytes = (double)a.k * Ty::kBytes, stages = ceil(kbytes / kStage);
+  auto rounds = [&](int ti, int tj) {
+    const double r = expected_tiles(a, l, tj) * ceil_div(a.n, ti) / cus;
+    return r <= 1 ? 1 : r + 0.3;
+  };
+  const double unit_128 = 0.78 - 0.195 * clamp01((l.rows - 128) / 128);
+  const double unit_64 = unit_128 * (0.5 + 0.085 * clamp01(l.rows / 128));
+  const double large = rounds(256, 256) * (stages + 3), middle = rounds(256, 128) * unit_128 * (stages + 4.2);
+  const double small = rounds(128, 128) * unit_64 * (stages + 5.4);
+  if constexpr (FORM == kNT) {
+    // Strips, where not even the small tiles occupy the GPU. Nanoseconds: a strip moves 30 bytes a ns
+    // into its CU, all of them 9200, weights from memory 6000; a small tile takes 300 to 430 a stage.
+    if (expected_tiles(a, l, 128) * ceil_div(a.n, 128) <= cus) {
+      auto strips = [&](int t) {
+        const double per = (t + (l.rows < t ? l.rows : t)) * kbytes;
+        const double all = expected_tiles(a, l, t) * ceil_div(a.n, t) * per, weights = l.groups * a.n * kbytes;
+        return 3500 + fmax(fmax(all / 9200, per / 30), weights / 6000);
+      };
+      const double one = strips(16), two = strips(32), tile = 9000 + stages * (300 + fmin(l.rows, 128));
+      if (fmin(one, two) < tile)
+        return one <= two ? launch_strips<Ty, Out, 1, 1>(a, s) : launch_strips<Ty, Out, 2, 2>(a, s);
+    }
+  }
+  if (large <= middle && large <= small)
+    return l.rows <= 512 ? launch_tiles<Ty, Out, FORM, 256, 256, true>(a, s)
+                         : launch_tiles<Ty, Out, FORM, 256, 256, false>(a, s);
+  if (middle <= small)
+    return l.rows <= 256 ? launch_tiles<Ty, Out, FORM, 256, 128, true>(a, s)
+                         : launch_tiles<Ty, Out, FORM, 256, 128, false>(a, s);
+  return l.rows <= 256 ? launch_tiles<Ty, Out, FORM, 128, 128, true>(a, s)
+                       : launch_tiles<Ty, Out, FORM, 128, 128, false>(a, s);
+}
+
+template <class In, int CHUNKS, bool ROW_WAVE>
+int launch_quantize_rows(int64_t rows, int cols, int64_t ldx, const In* x, int8_t* q, float* scale, hipStream_t s) {
+  const dim3 grid((unsigned)(ROW_WAVE ? ceil_div(rows, 4) : rows));
+  hipLaunchKernelGGL((k_quantize_int8<In, CHUNKS, ROW_WAVE>), grid, dim3(256), 0, s, rows, cols, ldx, x, q, scale);
+  return launched();
+}
+
+// Short rows go to a wavefront each (no barrier), longer ones to a workgroup each; CHUNKS is what
+// holds the row.
+template <class In>
+int launch_quantize(int64_t rows, int cols, int64_t ldx, const In* x, int8_t* q, float* scale, hipStream_t s) {
+  constexpr int kPer = 16 / (int)sizeof(In);
+  const int64_t count = cols / kPer, blocks = rows < kMaxBlocks ? rows : kMaxBlocks;
+  if (cols > 0 && chunks(x, ldx, cols, (int)sizeof(In)) && aligned(q, kPer) && count <= 8 * 256 && rows <= kMaxRowBlocks) {
+    if (count <= 64) return launch_quantize_rows<In, 1, true>(rows, cols, ldx, x, q, scale, s);
+    if (count <= 2 * 64) return launch_quantize_rows<In, 2, true>(rows, cols, ldx, x, q, scale, s);
+    if (count <= 256) return launch_quantize_rows<In, 1, false>(rows, cols, ldx, x, q, scale, s);
+    if (count <= 2 * 256) return launch_quantize_rows<In, 2, false>(rows, cols, ldx, x, q, scale, s);
+    if (count <= 4 * 256) return launch_quantize_rows<In, 4, false>(rows, cols, ldx, x, q, scale, s);
+    return launch_quantize_rows<In, 8, false>(rows, cols, ldx, x, q, scale, s);
+  }
+  hipLaunchKernelGGL((k_quantize_int8_any<In>), dim3((unsigned)blocks), dim3(256), 0, s, rows, cols, ldx, x, q, scale);
+  return launched();
 }
 
 template <class Ty>
@@ -932,11 +1263,15 @@ int product16(const megamoe_product* p, const Args& a, hipStream_t s) {
   return p->transposed ? launch_any<Ty, Out, true>(a, s) : launch_any<Ty, Out, false>(a, s);
 }
 
+// The large tiles wherever they occupy the GPU: four small ones write as much and read twice as much
+// (128 experts, 2048 by 768, 32768 rows: 206 us against 307; 8 experts, 1024 by 512, 150 rows, 64
+// large tiles: 15.5 us against 11.0).
 template <class Ty>
 int wgrad16(const Args& a, hipStream_t s) {
-  if (a.rows > 0 && chunks(a.x, a.ldx, a.k, 2) && chunks(a.w, a.ldy, a.n, 2))
-    return launch_tiles<Ty, typename Ty::Elem, kTN, 256>(a, s);
-  return launch_wgrad_any<Ty>(a, s);
+  if (!chunks(a.x, a.ldx, a.k, 2) || !chunks(a.w, a.ldy, a.n, 2)) return launch_wgrad_any<Ty>(a, s);
+  if (a.groups * ceil_div(a.n, 256) * ceil_div(a.k, 256) >= compute_units())
+    return launch_tiles<Ty, typename Ty::Elem, kTN, 256, 256, false>(a, s);
+  return launch_tiles<Ty, typename Ty::Elem, kTN, 128, 128, false>(a, s);
 }
 
 template <class Out>
@@ -1001,15 +1336,10 @@ int megamoe_quantize_rows_int8(int64_t rows, int32_t cols, int64_t ldx, int32_t 
   if (rows == 0) return MEGAMOE_OK;
   if (!scale || (cols && (!x || !q))) return MEGAMOE_ERR_INVALID_ARGUMENT;
   if (!aligned(x, dtype == MEGAMOE_FP32 ? 4 : 2) || !aligned(scale, 4)) return MEGAMOE_ERR_INVALID_ARGUMENT;
-  const dim3 grid((unsigned)(rows < kMaxBlocks ? rows : kMaxBlocks));
   hipStream_t s = (hipStream_t)stream;
-  if (dtype == MEGAMOE_BF16)
-    hipLaunchKernelGGL(k_quantize_int8<__bf16>, grid, dim3(256), 0, s, rows, cols, ldx, (const __bf16*)x, q, scale);
-  else if (dtype == MEGAMOE_FP16)
-    hipLaunchKernelGGL(k_quantize_int8<_Float16>, grid, dim3(256), 0, s, rows, cols, ldx, (const _Float16*)x, q, scale);
-  else
-    hipLaunchKernelGGL(k_quantize_int8<float>, grid, dim3(256), 0, s, rows, cols, ldx, (const float*)x, q, scale);
-  return launched();
+  if (dtype == MEGAMOE_BF16) return launch_quantize(rows, cols, ldx, (const __bf16*)x, q, scale, s);
+  if (dtype == MEGAMOE_FP16) return launch_quantize(rows, cols, ldx, (const _Float16*)x, q, scale, s);
+  return launch_quantize(rows, cols, ldx, (const float*)x, q, scale, s);
 }
 
 }  // extern "C"

@@ -25,49 +25,52 @@ import ctypes
 import torch
 
 from . import _lib
-from .submission import _on, _stream_handle
+from .submission import _stream_handle
 
 _TYPES = {torch.bfloat16: _lib.BF16, torch.float16: _lib.FP16, torch.float32: _lib.FP32}
-_byref = ctypes.byref
+_HALVES = {torch.bfloat16: _lib.BF16, torch.float16: _lib.FP16}
+_byref, _Product, _Tensor = ctypes.byref, _lib.Product, torch.Tensor
 
 
 def _device(t, name: str) -> torch.device:
-    if not isinstance(t, torch.Tensor):
+    if not isinstance(t, _Tensor):
         raise ValueError(f"{name}: expected a tensor")
-    if t.device.type != "cuda":
+    if not t.is_cuda:
         raise RuntimeError(f"the products run on a GPU; {name} is on {t.device}")
     return t.device
 
 
-def _dense(t, name: str, dtype, shape, device) -> None:
-    if not isinstance(t, torch.Tensor):
+def _dense(t, name: str, dtype, shape, index: int) -> None:
+    """``t`` is a contiguous tensor of this type and shape on GPU ``index``, or ValueError."""
+    if not isinstance(t, _Tensor):
         raise ValueError(f"{name}: expected a tensor")
-    if t.dtype != dtype or tuple(t.shape) != tuple(shape):
+    if t.dtype != dtype or t.shape != shape:
         raise ValueError(f"{name}: expected {tuple(shape)} {dtype}, got {tuple(t.shape)} {t.dtype}")
-    if t.device != device or not t.is_contiguous():
-        raise ValueError(f"{name}: must be contiguous on {device}")
+    if t.get_device() != index or not t.is_contiguous():
+        raise ValueError(f"{name}: must be contiguous on cuda:{index}")
 
 
 def _stride(t: torch.Tensor) -> int | None:
     """The row stride of 2-D ``t``, or None if its rows are not dense or overlap."""
     rows, cols = t.shape
-    if cols > 1 and t.stride(1) != 1:
+    ld, step = t.stride()
+    if step != 1 and cols > 1:
         return None
     if rows <= 1:
-        return max(cols, 1)
-    return t.stride(0) if t.stride(0) >= cols else None
+        return cols or 1
+    return ld if ld >= cols else None
 
 
-def _rows(t, name: str, dtype, cols, device) -> tuple[torch.Tensor, int]:
+def _rows(t, name: str, dtype, cols, index: int) -> tuple[torch.Tensor, int]:
     """2-D input rows and their stride; rows that are not dense (a broadcast or transposed
     tensor) are copied."""
-    if not isinstance(t, torch.Tensor):
+    if not isinstance(t, _Tensor):
         raise ValueError(f"{name}: expected a tensor")
     if t.dim() != 2 or t.dtype != dtype or (cols is not None and t.shape[1] != cols):
         raise ValueError(f"{name}: expected [rows, {'columns' if cols is None else cols}] {dtype}, "
                          f"got {tuple(t.shape)} {t.dtype}")
-    if t.device != device:
-        raise ValueError(f"{name}: on {t.device}, expected {device}")
+    if t.get_device() != index:
+        raise ValueError(f"{name}: on {t.device}, expected cuda:{index}")
     ld = _stride(t)
     if ld is None:
         t = t.contiguous()
@@ -83,14 +86,12 @@ def _extent(t: torch.Tensor) -> tuple[int, int]:
     return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
 
 
-def _result(out, shape, dtype, device, inputs) -> tuple[torch.Tensor, int]:
-    """The result's tensor and row stride; a given ``out`` may not overlap an input."""
-    if out is None:
-        return torch.empty(shape, dtype=dtype, device=device), max(shape[-1], 1)
-    if not isinstance(out, torch.Tensor):
+def _given(out, shape, dtype, index: int, inputs) -> int:
+    """The row stride of a given result, which may not overlap an input."""
+    if not isinstance(out, _Tensor):
         raise ValueError("out: expected a tensor")
-    if out.dtype != dtype or tuple(out.shape) != tuple(shape) or out.device != device:
-        raise ValueError(f"out: expected {tuple(shape)} {dtype} on {device}, got {tuple(out.shape)} {out.dtype} on "
+    if out.dtype != dtype or out.shape != shape or out.get_device() != index:
+        raise ValueError(f"out: expected {tuple(shape)} {dtype} on cuda:{index}, got {tuple(out.shape)} {out.dtype} on "
                          f"{out.device}")
     ld = _stride(out) if out.dim() == 2 else (max(shape[-1], 1) if out.is_contiguous() else None)
     if ld is None:
@@ -102,33 +103,42 @@ def _result(out, shape, dtype, device, inputs) -> tuple[torch.Tensor, int]:
         c, d = _extent(t)
         if a < d and c < b:
             raise ValueError("out: overlaps an input")
-    return out, ld
+    return ld
 
 
-def _run(fn, what: str, device: torch.device, *args) -> None:
-    stream = _stream_handle(device)
-    with _on(device):
-        status = fn(*args, stream)
+def _run(name: str, device: torch.device, *args) -> None:
+    """One call of the library on torch's current stream of ``device``."""
+    fn = getattr(_lib.load(), name)
+    if torch.cuda.current_device() == device.index:
+        status = fn(*args, _stream_handle(device))
+    else:
+        with torch.cuda.device(device):
+            status = fn(*args, _stream_handle(device))
     if status:
-        _lib.check(status, what)
+        _lib.check(status, name.removeprefix("megamoe_"))
 
 
 def _grouped(x, weight, counts, transposed: bool, out) -> torch.Tensor:
     device = _device(x, "x")
-    if x.dtype not in (torch.bfloat16, torch.float16):
-        raise ValueError(f"x: expected bfloat16 or float16, got {x.dtype}")
-    if not isinstance(weight, torch.Tensor) or weight.dim() != 3:
+    index, dtype = device.index, x.dtype
+    if dtype not in _HALVES:
+        raise ValueError(f"x: expected bfloat16 or float16, got {dtype}")
+    if not isinstance(weight, _Tensor) or weight.dim() != 3:
         raise ValueError("weight: expected [experts, out, in] (or [experts, in, out] when transposed)")
-    E = weight.shape[0]
-    N, K = (weight.shape[2], weight.shape[1]) if transposed else weight.shape[1:]
-    _dense(weight, "weight", x.dtype, weight.shape, device)
-    x, ldx = _rows(x, "x", x.dtype, K, device)
-    _dense(counts, "counts", torch.int64, (E,), device)
+    shape = weight.shape
+    E, N, K = shape
+    if transposed:
+        N, K = K, N
+    _dense(weight, "weight", dtype, shape, index)
+    x, ldx = _rows(x, "x", dtype, K, index)
+    _dense(counts, "counts", torch.int64, (E,), index)
     R = x.shape[0]
-    y, ldy = _result(out, (R, N), x.dtype, device, (x, weight, counts))
-    p = _lib.Product(R, E, N, K, _TYPES[x.dtype], int(transposed), int(out is None), ldx, ldy)
-    _run(_lib.load().megamoe_grouped_mm, "grouped_mm", device, _byref(p), x.data_ptr(), weight.data_ptr(),
-         counts.data_ptr(), y.data_ptr())
+    if out is None:
+        y, ldy = x.new_empty((R, N)), N or 1
+    else:
+        y, ldy = out, _given(out, (R, N), dtype, index, (x, weight, counts))
+    p = _Product(R, E, N, K, _HALVES[dtype], transposed, out is None, ldx, ldy)
+    _run("megamoe_grouped_mm", device, _byref(p), x.data_ptr(), weight.data_ptr(), counts.data_ptr(), y.data_ptr())
     return y
 
 
@@ -172,41 +182,55 @@ def grouped_mm_wgrad(dy: torch.Tensor, x: torch.Tensor, counts: torch.Tensor, *,
     expert's rows (dy [R, N], x [R, K]; exchange them for a transposed weight). Experts without
     rows get zero."""
     device = _device(x, "x")
-    if x.dtype not in (torch.bfloat16, torch.float16):
-        raise ValueError(f"x: expected bfloat16 or float16, got {x.dtype}")
-    x, ldx = _rows(x, "x", x.dtype, None, device)
-    dy, ldy = _rows(dy, "dy", x.dtype, None, device)
-    if dy.shape[0] != x.shape[0]:
-        raise ValueError(f"dy: {dy.shape[0]} rows, x has {x.shape[0]}")
-    if not isinstance(counts, torch.Tensor) or counts.dim() != 1:
+    index, dtype = device.index, x.dtype
+    if dtype not in _HALVES:
+        raise ValueError(f"x: expected bfloat16 or float16, got {dtype}")
+    x, ldx = _rows(x, "x", dtype, None, index)
+    dy, ldy = _rows(dy, "dy", dtype, None, index)
+    R, K = x.shape
+    if dy.shape[0] != R:
+        raise ValueError(f"dy: {dy.shape[0]} rows, x has {R}")
+    if not isinstance(counts, _Tensor) or counts.dim() != 1:
         raise ValueError("counts: expected int64 [experts]")
-    E, N, K = counts.shape[0], dy.shape[1], x.shape[1]
-    _dense(counts, "counts", torch.int64, (E,), device)
-    dw, _ = _result(out, (E, N, K), x.dtype, device, (x, dy, counts))
-    p = _lib.Product(x.shape[0], E, N, K, _TYPES[x.dtype], 0, 0, ldx, ldy)
-    _run(_lib.load().megamoe_grouped_mm_wgrad, "grouped_mm_wgrad", device, _byref(p), dy.data_ptr(), x.data_ptr(),
-         counts.data_ptr(), dw.data_ptr())
+    E, N = counts.shape[0], dy.shape[1]
+    _dense(counts, "counts", torch.int64, (E,), index)
+    if out is None:
+        dw = x.new_empty((E, N, K))
+    else:
+        dw = out
+        _given(out, (E, N, K), dtype, index, (x, dy, counts))
+    p = _Product(R, E, N, K, _HALVES[dtype], 0, 0, ldx, ldy)
+    _run("megamoe_grouped_mm_wgrad", device, _byref(p), dy.data_ptr(), x.data_ptr(), counts.data_ptr(), dw.data_ptr())
     return dw
 
 
-def _int8(x, x_scale, weight, weight_scale, counts, out_dtype, out, what: str) -> torch.Tensor:
+def _int8(x, x_scale, weight, weight_scale, counts, out_dtype, out) -> torch.Tensor:
     device = _device(x, "x")
-    if out_dtype not in _TYPES:
+    index = device.index
+    kind = _TYPES.get(out_dtype)
+    if kind is None:
         raise ValueError(f"out_dtype: expected bfloat16, float16 or float32, got {out_dtype}")
-    K, N = weight.shape[-1], weight.shape[-2]
-    E = weight.shape[0] if counts is not None else 1
-    x, ldx = _rows(x, "x", torch.int8, K, device)
+    shape = weight.shape
+    N, K = shape[-2:]
+    x, ldx = _rows(x, "x", torch.int8, K, index)
     R = x.shape[0]
-    _dense(x_scale, "x_scale", torch.float32, (R,), device)
-    _dense(weight, "weight", torch.int8, weight.shape, device)
-    _dense(weight_scale, "weight_scale", torch.float32, weight.shape[:-1], device)
-    if counts is not None:
-        _dense(counts, "counts", torch.int64, (E,), device)
-    y, ldy = _result(out, (R, N), out_dtype, device,
-                     [t for t in (x, x_scale, weight, weight_scale, counts) if t is not None])
-    p = _lib.Product(R, E, N, K, _TYPES[out_dtype], 0, int(out is None), ldx, ldy)
-    _run(_lib.load().megamoe_int8_mm, what, device, _byref(p), x.data_ptr(), x_scale.data_ptr(), weight.data_ptr(),
-         weight_scale.data_ptr(), None if counts is None else counts.data_ptr(), y.data_ptr())
+    _dense(x_scale, "x_scale", torch.float32, (R,), index)
+    _dense(weight, "weight", torch.int8, shape, index)
+    _dense(weight_scale, "weight_scale", torch.float32, shape[:-1], index)
+    if counts is None:
+        E, counts_at = 1, None
+    else:
+        E = shape[0]
+        _dense(counts, "counts", torch.int64, (E,), index)
+        counts_at = counts.data_ptr()
+    if out is None:
+        y, ldy = torch.empty((R, N), dtype=out_dtype, device=device), N or 1
+    else:
+        inputs = (x, x_scale, weight, weight_scale) + (() if counts is None else (counts,))
+        y, ldy = out, _given(out, (R, N), out_dtype, index, inputs)
+    p = _Product(R, E, N, K, kind, 0, out is None, ldx, ldy)
+    _run("megamoe_int8_mm", device, _byref(p), x.data_ptr(), x_scale.data_ptr(), weight.data_ptr(),
+         weight_scale.data_ptr(), counts_at, y.data_ptr())
     return y
 
 
@@ -218,7 +242,7 @@ def int8_mm(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, weight
     _device(x, "x")
     if not isinstance(weight, torch.Tensor) or weight.dim() != 2:
         raise ValueError("weight: expected int8 [out, in]")
-    return _int8(x, x_scale, weight, weight_scale, None, out_dtype, out, "int8_mm")
+    return _int8(x, x_scale, weight, weight_scale, None, out_dtype, out)
 
 
 def grouped_int8_mm(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor,
@@ -231,7 +255,7 @@ def grouped_int8_mm(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor
         raise ValueError("weight: expected int8 [experts, out, in]")
     if not isinstance(counts, torch.Tensor):
         raise ValueError("counts: expected int64 [experts]")
-    return _int8(x, x_scale, weight, weight_scale, counts, out_dtype, out, "grouped_int8_mm")
+    return _int8(x, x_scale, weight, weight_scale, counts, out_dtype, out)
 
 
 def quantize_rows_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
@@ -239,12 +263,12 @@ def quantize_rows_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     largest magnitude (at least 2^-100), scale = a / 127 and q = x * (127 / a) rounded to nearest
     even. A row with NaN or an infinity gets the scale NaN and zeros."""
     device = _device(x, "x")
-    if x.dtype not in _TYPES or x.dim() != 2:
+    kind = _TYPES.get(x.dtype)
+    if kind is None or x.dim() != 2:
         raise ValueError("quantize_rows_int8 takes 2-D bfloat16, float16 or float32 rows")
-    x, ld = _rows(x, "x", x.dtype, None, device)
-    rows, cols = x.shape
-    q = torch.empty((rows, cols), dtype=torch.int8, device=device)
+    x, ld = _rows(x, "x", x.dtype, None, device.index)
+    rows, cols = shape = x.shape
+    q = torch.empty(shape, dtype=torch.int8, device=device)
     scale = torch.empty((rows,), dtype=torch.float32, device=device)
-    _run(_lib.load().megamoe_quantize_rows_int8, "quantize_rows_int8", device, rows, cols, ld, _TYPES[x.dtype],
-         x.data_ptr(), q.data_ptr(), scale.data_ptr())
+    _run("megamoe_quantize_rows_int8", device, rows, cols, ld, kind, x.data_ptr(), q.data_ptr(), scale.data_ptr())
     return q, scale
