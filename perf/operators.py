@@ -17,6 +17,7 @@ sizes.
 
 from __future__ import annotations
 
+import functools
 import hashlib
 import importlib
 import math
@@ -39,6 +40,7 @@ TRAINED = ("tiny", "qwen3")  # geometries whose training step is drawn
 DTYPES = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
 
 
+@functools.lru_cache(maxsize=None)  # a program imports the package once
 def _products():
     import __graft_entry__
 
