@@ -35,8 +35,8 @@ enum megamoe_product_type {
 };
 
 /* Geometry of one product. Limits beyond which MEGAMOE_ERR_UNSUPPORTED is returned: groups
- * 1024, rows 2^31 - 1, row strides 8 MiB, and 131071 for k of an int8 product (its int32 sums
- * cannot overflow up to there). */
+ * 1024, rows 2^30, row strides 4 MiB (ldx, and ldy as if its elements had four bytes), and 131071
+ * for k of an int8 product (its int32 sums cannot overflow up to there). */
 typedef struct megamoe_product {
   int64_t rows;       /* rows of x and y, >= 0 */
   int32_t groups;     /* E >= 1 */

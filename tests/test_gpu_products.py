@@ -6,6 +6,7 @@ int32) in any order, so the result has to equal the 64-bit one rounded once, bit
 
 from __future__ import annotations
 
+import re
 import sys
 
 import pytest
@@ -200,6 +201,26 @@ def _exact_dx(dy, wt, counts):
     return _product(dy, wt.transpose(1, 2).contiguous(), counts, True)
 
 
+@pytest.mark.parametrize("transposed", (False, True), ids=("nk", "kn"))
+def test_second_derivatives(transposed):
+    """The gradients are bilinear like the product: of <dx, v> and <dw, u> the derivatives are again
+    products of the same kind, on these whole numbers exact."""
+    counts, c, K, N = [5, 0, 9], _counts([5, 0, 9]), 40, 24
+    x, dy = _whole((14, K), BF16, 140, most=1).requires_grad_(), _whole((14, N), BF16, 141, most=1).requires_grad_()
+    w = _whole((3, K, N) if transposed else (3, N, K), BF16, 142, most=1).requires_grad_()
+    v, u = _whole((14, K), BF16, 143, most=1), _whole(w.shape, BF16, 144, most=1)
+    y = products.grouped_mm(x, w, c, transposed=transposed)
+    dx, dw = torch.autograd.grad(y, (x, w), dy, create_graph=True)
+    by_dy, by_w = torch.autograd.grad(dx, (dy, w), v, retain_graph=True)
+    back_dy, by_x = torch.autograd.grad(dw, (dy, x), u)
+    with torch.no_grad():
+        turned = lambda t: t.transpose(1, 2) if transposed else t  # noqa: E731
+        _same(by_dy, _product(v, w, counts, transposed), "<dx, v> by dy")
+        _same(by_w, turned(_wgrad(dy, v, counts)), "<dx, v> by w")
+        _same(back_dy, _product(x, u, counts, transposed), "<dw, u> by dy")
+        _same(by_x, _product(dy, u, counts, not transposed), "<dw, u> by x")
+
+
 def test_gradient_of_broadcast_rows_and_of_one_input():
     """A result summed to a number hands back a broadcast gradient; x itself may be a broadcast
     row; and only the gradient that is asked for is made."""
@@ -326,6 +347,87 @@ def test_long_offsets():
     dy[-2:] = _whole((2, 16), BF16, 36)
     _same(products.grouped_mm_wgrad(dy, x, _counts([R - 2, 2]))[1], dy[-2:].double().T.contiguous() @ x[-2:].double(),
           "wgrad rows")
+
+
+# Calls that the rules send to each kernel: (counts, K, N), with each of them the tiles and whether
+# the weights go past the caches, in the form y = x w^T and in y = x w.
+SIZES = {
+    (256, 256, True): ([90, 110, 0, 200] * 16, 256, 520), (256, 256, False): ([3900, 4100], 256, 1032),
+    (256, 128, True): ([4, 12, 0, 16] * 2, 256, 6144), (256, 128, False): ([4100, 3900], 256, 520),
+    (128, 128, True): ([2, 1, 5, 0] * 16, 256, 520), (128, 128, False): ([300, 500] * 4, 256, 1032),
+}
+
+
+def _kernels(call):
+    """(kernel, its type, its numbers) of every products kernel that ``call`` launches, from the profiler's names,
+    demangled or not."""
+    call()
+    torch.cuda.synchronize()
+    with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CUDA]) as prof:
+        call()
+        torch.cuda.synchronize()
+    found = set()
+    for e in prof.events():
+        kernel = re.search(r"k_(tiles|strips|product_any|wgrad_any|quantize_int8_any|quantize_int8)", e.name)
+        if kernel:
+            kind = re.search(r"Bf16|Fp16|Int8", e.name)
+            plain = e.name.replace("true", "1").replace("false", "0")
+            numbers = re.findall(r"(?<=L[ib])\d+(?=E)|(?<=FormE)\d(?=E)|(?<=[ )])\d+(?=[,>])", plain)
+            found.add((kernel.group(1), kind.group(0) if kind else "", tuple(int(n) for n in numbers)[-3:]))
+    return found
+
+
+def _reached(kernel, kind, numbers, call):
+    """Whether ``call`` launches it. Demangled names can lose the first numbers, but not the last ones' order."""
+    return any(name == kernel and k == kind and n == numbers[len(numbers) - len(n):] for name, k, n in _kernels(call))
+
+
+@pytest.mark.parametrize("dtype", (BF16, FP16, torch.int8), ids=("bf16", "fp16", "int8"))
+@pytest.mark.parametrize("size", SIZES, ids=lambda s: f"{s[0]}x{s[1]}{'-once' if s[2] else ''}")
+def test_every_tile_size_is_reached_and_exact(size, dtype):
+    counts, K, N = SIZES[size]
+    kind = {BF16: "Bf16", FP16: "Fp16", torch.int8: "Int8"}[dtype]
+    _log(f"{size} {dtype}: {sum(counts)} rows of {len(counts)} experts, K={K} N={N}")
+    x, c = _whole((sum(counts) + 3, K), dtype, 150, most=3), _counts(counts)
+    if dtype == torch.int8:
+        w, one = _whole((len(counts), N, K), dtype, 151, most=3), torch.ones(len(x), device=DEV)
+        ws = torch.ones((len(counts), N), device=DEV)
+        for out_dtype in (BF16, FP16, FP32):
+            call = lambda: products.grouped_int8_mm(x, one, w, ws, c, out_dtype=out_dtype)  # noqa: E731
+            assert _reached("tiles", kind, size, call)
+            _same(call(), _product(x, w, counts).float(), f"y {out_dtype}")
+        return
+    for transposed in (False, True):
+        w = _whole((len(counts), K, N) if transposed else (len(counts), N, K), dtype, 151, most=3)
+        call = lambda: products.grouped_mm(x, w, c, transposed=transposed)  # noqa: E731
+        assert _reached("tiles", kind, size, call)
+        _same(call(), _product(x, w, counts, transposed), "y")
+
+
+def test_the_other_kernels_are_reached():
+    """Strips of both sizes, both tile sizes of the weights' gradient, the kernels of any alignment."""
+    for dtype, kind in ((BF16, "Bf16"), (FP16, "Fp16")):
+        for counts, K, N, strip in (([1] * 8, 2048, 768, (1, 1)), ([256], 2048, 768, (2, 2))):
+            x, w, c = _whole((sum(counts), K), dtype, 152), _whole((len(counts), N, K), dtype, 153), _counts(counts)
+            assert _reached("strips", kind, strip, lambda: products.grouped_mm(x, w, c))
+            _same(products.grouped_mm(x, w, c), _product(x, w, counts), "y")
+        for counts, K, N, size in (([30] * 20, 1024, 1000, (256, 256)), ([30, 5], 512, 520, (128, 128))):
+            x, dy, c = _whole((sum(counts), K), dtype, 154), _whole((sum(counts), N), dtype, 155), _counts(counts)
+            assert _reached("tiles", kind, (*size, 0), lambda: products.grouped_mm_wgrad(dy, x, c))
+            _same(products.grouped_mm_wgrad(dy, x, c), _wgrad(dy, x, counts), "dw")
+        x, w, c = _whole((5, 33), dtype, 156), _whole((1, 9, 33), dtype, 157), _counts([5])
+        names = _kernels(lambda: (products.grouped_mm(x, w, c), products.grouped_mm_wgrad(_whole((5, 9), dtype, 1), x, c)))
+        assert {n[:2] for n in names} == {("product_any", kind), ("wgrad_any", kind)}
+    one = torch.ones(256, device=DEV)
+    for M, strip in ((1, (1, 1)), (256, (2, 2))):
+        x, w = _whole((M, 2048), torch.int8, 158), _whole((768, 2048), torch.int8, 159)
+        assert _reached("strips", "Int8", strip, lambda: products.int8_mm(x, one[:M], w, torch.ones(768, device=DEV)))
+    for dtype in (BF16, FP16, FP32):
+        wide = 16 // dtype.itemsize
+        for chunks, kernel in ((64, (1, 1)), (128, (2, 1)), (256, (1, 0)), (512, (2, 0)), (1024, (4, 0)), (2048, (8, 0))):
+            x = _whole((3, chunks * wide), dtype, 160)
+            assert _reached("quantize_int8", "", kernel, lambda: products.quantize_rows_int8(x))
+        assert _reached("quantize_int8_any", "", (), lambda: products.quantize_rows_int8(_whole((3, 33), dtype, 1)))
 
 
 # ---------------------------------------------------------------------------------------

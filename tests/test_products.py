@@ -36,8 +36,8 @@ GEOMETRY = [
     (dict(rows=-1), _lib.ERR_SHAPE), (dict(groups=0), _lib.ERR_SHAPE), (dict(n=-1), _lib.ERR_SHAPE),
     (dict(k=-8), _lib.ERR_SHAPE), (dict(ldx=31), _lib.ERR_SHAPE), (dict(ldy=63), _lib.ERR_SHAPE),
     (dict(dtype=-1), _lib.ERR_SHAPE), (dict(dtype=3), _lib.ERR_SHAPE),
-    (dict(groups=1025), _lib.ERR_UNSUPPORTED), (dict(rows=1 << 31), _lib.ERR_UNSUPPORTED),
-    (dict(ldx=(8 << 20) + 1), _lib.ERR_UNSUPPORTED), (dict(ldy=(8 << 20) + 1), _lib.ERR_UNSUPPORTED),
+    (dict(groups=1025), _lib.ERR_UNSUPPORTED), (dict(rows=(1 << 30) + 1), _lib.ERR_UNSUPPORTED),
+    (dict(ldx=(4 << 20) + 1), _lib.ERR_UNSUPPORTED), (dict(ldy=(1 << 20) + 1), _lib.ERR_UNSUPPORTED),
 ]
 
 

@@ -463,7 +463,9 @@ struct Side {
   }
 };
 
-constexpr uint32_t kOutside = 0xC0000000u;  // an offset past every buffer resource
+// An offset past every buffer resource (256 rows of kMaxStrideBytes), also with the loads' largest
+// second offset (192 rows and a row) added.
+constexpr uint32_t kOutside = 0x80000000u;
 
 template <class T>
 __device__ __forceinline__ T uniform(T v) {
@@ -476,23 +478,37 @@ __device__ __forceinline__ T uniform(T v) {
   }
 }
 
+// The buffer resource of the `bytes` bytes from `base`.
+__device__ __forceinline__ i32x4 resource(const void* base, uint32_t bytes) {
+  const uint64_t b = (uint64_t)uniform((const uint8_t*)base);
+  return i32x4{(int)(uint32_t)b, (int)((uint32_t)(b >> 32) & 0xffffu), (int)uniform(bytes), 0x00020000};
+}
+
 // 16 bytes a lane into LDS (1024 consecutive ones from byte address `to`), from `base` + at +
-// along; zero from `bytes` on.
+// along; zero from `bytes` on. ONCE: past the caches.
 template <bool ONCE>
 __device__ __forceinline__ void load_lds(uint32_t to, const uint8_t* base, uint32_t bytes, uint32_t at, uint32_t along) {
 #ifdef __HIP_DEVICE_COMPILE__
-  const uint64_t b = (uint64_t)uniform(base);
-  const i32x4 rsrc = {(int)(uint32_t)b, (int)((uint32_t)(b >> 32) & 0xffffu), (int)uniform(bytes), 0x00020000};
   if constexpr (ONCE)
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen nt lds"
                  :
-                 : "s"(uniform(to)), "v"(at), "s"(rsrc), "s"(uniform(along))
+                 : "s"(uniform(to)), "v"(at), "s"(resource(base, bytes)), "s"(uniform(along))
                  : "memory", "m0");
   else
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
                  :
-                 : "s"(uniform(to)), "v"(at), "s"(rsrc), "s"(uniform(along))
+                 : "s"(uniform(to)), "v"(at), "s"(resource(base, bytes)), "s"(uniform(along))
                  : "memory", "m0");
+#endif
+}
+
+// The same with 4 bytes a lane: `count` floats (up to 64, zero behind them).
+__device__ __forceinline__ void load_floats(uint32_t to, const float* base, int count) {
+#ifdef __HIP_DEVICE_COMPILE__
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
+               :
+               : "s"(uniform(to)), "v"((threadIdx.x & 63) * 4), "s"(resource(base, (uint32_t)max(count, 0) * 4))
+               : "memory", "m0");
 #endif
 }
 
@@ -606,6 +622,7 @@ struct Work {
   int group, first, last;  // rows of y (the products), of the group (the weights' gradient)
   int i0, j0;              // first column and row of the output tile (j0: within rows first..last)
   int stages;
+  int place;               // of its scales
   int turn;                // the stage that comes first (c is walked in a circle)
   uint32_t rows_a, rows_b;  // bytes of the rows that exist (c contiguous)
 };
@@ -623,6 +640,8 @@ __global__ __launch_bounds__(kThreads, 2) void k_tiles(Args p) {
   constexpr int kC = kStage / Ty::kBytes;  // c of one stage
   __shared__ __align__(1024) uint8_t lds[BUFFERS * kBytes];
   __shared__ Table table;
+  // The int8 product's scales of two tiles' i and j, loaded with the tile's first stage.
+  __shared__ float scales[2][Ty::kBytes == 1 ? TI + TJ : 1];
 
   const int wave = uniform((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int wi = wave % WI, wj = wave / WI;
@@ -642,8 +661,8 @@ __global__ __launch_bounds__(kThreads, 2) void k_tiles(Args p) {
   const int row_tiles = FORM == kTN ? p.groups * ((p.n + TJ - 1) / TJ)
                                     : uniform((int)(table.tiles[kMaxGroups] + table.small[kMaxGroups]));
   const int total = row_tiles * tiles_i;
-  if (FORM != kTN && p.fill_rest)
-    for (int64_t r = used + blockIdx.x; r < p.rows; r += gridDim.x)
+  if (FORM != kTN && p.fill_rest)  // the last workgroups first: the ones that may have no tile
+    for (int64_t r = used + (gridDim.x - 1 - blockIdx.x); r < p.rows; r += gridDim.x)
       for (int i = threadIdx.x; i < ni; i += kThreads) out[r * ldo + i] = (Out)0.f;
 
   const int64_t lda = (int64_t)Ty::kBytes * (FORM == kNT ? p.k : FORM == kNN ? p.n : p.ldx);
@@ -685,6 +704,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_tiles(Args p) {
   int tile = xcd_tile(step, total);
   if (tile < 0) return;
   Work ahead = locate_work(tile);  // the tile that is being loaded
+  ahead.place = 0;
   Work now = ahead;                // the tile that is being multiplied
   int stage = 0;                   // of `ahead`
   bool more = true;
@@ -701,6 +721,17 @@ __global__ __launch_bounds__(kThreads, 2) void k_tiles(Args p) {
     return s >= ahead.stages && more ? s - ahead.stages : s;
   };
   auto load_a = [&](auto i, int buf) {
+    if constexpr (Ty::kBytes == 1 && i.value == 0) {
+      if (stage == 0 && more) {
+        const uint32_t at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) float*)scales[ahead.place];
+        if (wave < TI / 64)
+          load_floats(at + 256 * wave, p.sw + (size_t)ahead.group * p.n + ahead.i0 + 64 * wave,
+                      min(p.n - ahead.i0 - 64 * wave, 64));
+        const int part = wave - (8 - TJ / 64);
+        if (part >= 0)
+          load_floats(at + 4 * TI + 256 * part, p.sx + ahead.first + 64 * part, min(ahead.last - ahead.first - 64 * part, 64));
+      }
+    }
     const int stage = at_stage();
     const uint32_t to = lds0 + buf * kBytes;
     if constexpr (kAcol) {
@@ -732,10 +763,12 @@ __global__ __launch_bounds__(kThreads, 2) void k_tiles(Args p) {
     stage = 0;
     tile = xcd_tile(++step, total);
     more = tile >= 0;
+    const int place = ahead.place ^ 1;
     if (more)
       ahead = locate_work(tile);
     else
       ahead.rows_a = ahead.rows_b = 0;
+    ahead.place = place;
   };
 
   typename Ty::Acc acc[FA][FB];
@@ -769,14 +802,12 @@ __global__ __launch_bounds__(kThreads, 2) void k_tiles(Args p) {
     for (int t = 0; t < FB; ++t) {
       const int j = now.j0 + wj * (TJ / WJ) + 16 * t + (lane & 15);
       float sx = 0.f;
-      if constexpr (Ty::kBytes == 1) sx = j < nj ? p.sx[now.first + j] : 0.f;
+      if constexpr (Ty::kBytes == 1) sx = scales[now.place][TI + wj * (TJ / WJ) + 16 * t + (lane & 15)];
       auto value = [&](int f, int e) {
-        if constexpr (Ty::kBytes == 1) {
-          const int i = now.i0 + wi * (TI / WI) + 16 * f + 4 * (lane >> 4) + e;
-          return scaled(acc[f][t][e], sx, i < ni ? p.sw[(size_t)now.group * p.n + i] : 0.f);
-        } else {
+        if constexpr (Ty::kBytes == 1)
+          return scaled(acc[f][t][e], sx, scales[now.place][wi * (TI / WI) + 16 * f + 4 * (lane >> 4) + e]);
+        else
           return acc[f][t][e];
-        }
       };
       auto put = [&](int i, OutN v) {
         if (j >= nj) return;
@@ -1061,7 +1092,7 @@ __global__ __launch_bounds__(256) void k_quantize_int8_any(int64_t rows, int col
 // Host
 // ---------------------------------------------------------------------------------------
 
-constexpr int64_t kMaxStrideBytes = 8 << 20, kMaxBlocks = 1 << 20, kMaxRowBlocks = 1 << 23;  // (a grid holds fewer than 2^32 threads)
+constexpr int64_t kMaxRows = 1 << 30, kMaxStrideBytes = 4 << 20, kMaxBlocks = 1 << 20, kMaxRowBlocks = 1 << 23;  // (a grid holds fewer than 2^32 threads)
 
 int launched() { return hipGetLastError() == hipSuccess ? MEGAMOE_OK : MEGAMOE_ERR_HIP; }
 
@@ -1069,7 +1100,7 @@ int check(const megamoe_product* p, int elem, bool wide_out) {
   if (!p) return MEGAMOE_ERR_INVALID_ARGUMENT;
   if (p->rows < 0 || p->groups < 1 || p->n < 0 || p->k < 0 || p->ldx < p->k || p->ldy < p->n) return MEGAMOE_ERR_SHAPE;
   if (p->dtype < MEGAMOE_BF16 || p->dtype > (wide_out ? MEGAMOE_FP32 : MEGAMOE_FP16)) return MEGAMOE_ERR_SHAPE;
-  if (p->groups > kMaxGroups || p->rows > INT32_MAX) return MEGAMOE_ERR_UNSUPPORTED;
+  if (p->groups > kMaxGroups || p->rows > kMaxRows) return MEGAMOE_ERR_UNSUPPORTED;
   if (p->ldx > kMaxStrideBytes / elem || p->ldy > kMaxStrideBytes / 4) return MEGAMOE_ERR_UNSUPPORTED;
   return MEGAMOE_OK;
 }
@@ -1173,11 +1204,11 @@ Load expected(const Args& a) {
   return Load{hit, a.rows / hit};
 }
 
-// Row tiles of `height` to expect: one of a group of up to half the height, half a tile more than
-// full ones of larger groups.
+// Row tiles of `height` to expect where groups' rows are spread like a geometric distribution: one
+// of a small group, half a tile more than full ones of a large one.
 double expected_tiles(const Args& a, const Load& l, int height) {
   if (!a.counts) return (double)ceil_div(a.rows, height);
-  return l.groups * (l.rows <= height / 2 ? 1.0 : l.rows / height + 0.5);
+  return l.groups / (1.0 - exp(-height / l.rows));
 }
 
 double clamp01(double v) { return v < 0 ? 0 : v > 1 ? 1 : v; }

@@ -142,45 +142,7 @@ def _grouped(x, weight, counts, transposed: bool, out) -> torch.Tensor:
     return y
 
 
-class _GroupedMM(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, counts, transposed):
-        ctx.save_for_backward(x, weight, counts)
-        ctx.transposed = transposed
-        return _grouped(x, weight, counts, transposed, None)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy):
-        x, weight, counts = ctx.saved_tensors
-        dx = _grouped(dy, weight, counts, not ctx.transposed, None) if ctx.needs_input_grad[0] else None
-        dw = None
-        if ctx.needs_input_grad[1]:
-            dw = grouped_mm_wgrad(x, dy, counts) if ctx.transposed else grouped_mm_wgrad(dy, x, counts)
-        return dx, dw, None, None
-
-
-def grouped_mm(x: torch.Tensor, weight: torch.Tensor, counts: torch.Tensor, *, transposed: bool = False,
-               out: torch.Tensor | None = None) -> torch.Tensor:
-    """y [R, N]: row r of expert e is ``weight[e] @ x[r]`` (weight [E, N, K]) or, ``transposed``,
-    ``x[r] @ weight[e]`` (weight [E, K, N]); bf16 or fp16, summed in fp32, rounded once.
-
-    ``x`` [R, K] may have any row stride (rows that are not dense are copied); ``weight`` is
-    dense. Differentiable in ``x`` and ``weight`` (once) unless ``out`` is given, which takes the
-    result and keeps its rows of no expert."""
-    if torch.is_grad_enabled() and ((isinstance(x, torch.Tensor) and x.requires_grad) or
-                                    (isinstance(weight, torch.Tensor) and weight.requires_grad)):
-        if out is not None:
-            raise ValueError("out: the result of inputs that require gradients cannot be written to a given tensor")
-        return _GroupedMM.apply(x, weight, counts, bool(transposed))
-    return _grouped(x, weight, counts, bool(transposed), out)
-
-
-def grouped_mm_wgrad(dy: torch.Tensor, x: torch.Tensor, counts: torch.Tensor, *,
-                     out: torch.Tensor | None = None) -> torch.Tensor:
-    """dw [E, N, K]: the gradient of ``grouped_mm``'s weight, ``dy[r]^T x[r]`` summed over each
-    expert's rows (dy [R, N], x [R, K]; exchange them for a transposed weight). Experts without
-    rows get zero."""
+def _wgrad(dy, x, counts, out) -> torch.Tensor:
     device = _device(x, "x")
     index, dtype = device.index, x.dtype
     if dtype not in _HALVES:
@@ -202,6 +164,75 @@ def grouped_mm_wgrad(dy: torch.Tensor, x: torch.Tensor, counts: torch.Tensor, *,
     p = _Product(R, E, N, K, _HALVES[dtype], 0, 0, ldx, ldy)
     _run("megamoe_grouped_mm_wgrad", device, _byref(p), dy.data_ptr(), x.data_ptr(), counts.data_ptr(), dw.data_ptr())
     return dw
+
+
+# The product and the weight's gradient are bilinear and each other's derivatives: the gradients
+# of either are again one of the two, so both can be differentiated any number of times.
+
+class _GroupedMM(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, counts, transposed):
+        ctx.save_for_backward(x, weight, counts)
+        ctx.transposed = transposed
+        return _grouped(x, weight, counts, transposed, None)
+
+    @staticmethod
+    def backward(ctx, dy):
+        x, weight, counts = ctx.saved_tensors
+        wants_x, wants_w, _, _ = ctx.needs_input_grad
+        dx = grouped_mm(dy, weight, counts, transposed=not ctx.transposed) if wants_x else None
+        dw = None
+        if wants_w:
+            dw = grouped_mm_wgrad(x, dy, counts) if ctx.transposed else grouped_mm_wgrad(dy, x, counts)
+        return dx, dw, None, None
+
+
+class _WGrad(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, dy, x, counts):
+        ctx.save_for_backward(dy, x, counts)
+        return _wgrad(dy, x, counts, None)
+
+    @staticmethod
+    def backward(ctx, g):
+        dy, x, counts = ctx.saved_tensors
+        g = g.contiguous()
+        wants_dy, wants_x, _ = ctx.needs_input_grad
+        return (grouped_mm(x, g, counts) if wants_dy else None,
+                grouped_mm(dy, g, counts, transposed=True) if wants_x else None, None)
+
+
+def _differentiable(out, *tensors) -> bool:
+    """Whether a call on ``tensors`` is to be recorded; it cannot write to a given tensor then."""
+    if not torch.is_grad_enabled() or not any(isinstance(t, _Tensor) and t.requires_grad for t in tensors):
+        return False
+    if out is not None:
+        raise ValueError("out: the result of inputs that require gradients cannot be written to a given tensor")
+    return True
+
+
+def grouped_mm(x: torch.Tensor, weight: torch.Tensor, counts: torch.Tensor, *, transposed: bool = False,
+               out: torch.Tensor | None = None) -> torch.Tensor:
+    """y [R, N]: row r of expert e is ``weight[e] @ x[r]`` (weight [E, N, K]) or, ``transposed``,
+    ``x[r] @ weight[e]`` (weight [E, K, N]); bf16 or fp16, summed in fp32, rounded once.
+
+    ``x`` [R, K] may have any row stride (rows that are not dense are copied); ``weight`` is
+    dense. Differentiable in ``x`` and ``weight`` unless ``out`` is given, which takes the result
+    and keeps its rows of no expert."""
+    if _differentiable(out, x, weight):
+        return _GroupedMM.apply(x, weight, counts, bool(transposed))
+    return _grouped(x, weight, counts, bool(transposed), out)
+
+
+def grouped_mm_wgrad(dy: torch.Tensor, x: torch.Tensor, counts: torch.Tensor, *,
+                     out: torch.Tensor | None = None) -> torch.Tensor:
+    """dw [E, N, K]: the gradient of ``grouped_mm``'s weight, ``dy[r]^T x[r]`` summed over each
+    expert's rows (dy [R, N], x [R, K]; exchange them for a transposed weight), bf16 or fp16, summed
+    in fp32. Experts without rows get zero. Differentiable in ``dy`` and ``x`` unless ``out`` is
+    given."""
+    if _differentiable(out, dy, x):
+        return _WGrad.apply(dy, x, counts)
+    return _wgrad(dy, x, counts, out)
 
 
 def _int8(x, x_scale, weight, weight_scale, counts, out_dtype, out) -> torch.Tensor:
