@@ -627,15 +627,23 @@ struct Work {
   uint32_t rows_a, rows_b;  // bytes of the rows that exist (c contiguous)
 };
 
+// Workgroups of a CU: two where tiles are mostly their start and their end, the small ones of the
+// weights' gradient, so that one of them multiplies while the other stores (13 experts, 1736 by 1000,
+// 1235 rows: 41.9 us with one that loads further ahead, 29.2 with two; 8 experts, 1024 by 512, 64 rows:
+// 10.8 and 9.1). The products want the loads further ahead (4096 by 4096, 512 rows: 36.8 us against
+// 46.0).
+template <Form FORM, int TI>
+constexpr int kPerCu = FORM == kTN && TI == 128 ? 2 : 1;
+
 template <class Ty, class Out, Form FORM, int TI, int TJ, bool ONCE>
-__global__ __launch_bounds__(kThreads, 2) void k_tiles(Args p) {
+__global__ __launch_bounds__(kThreads, 2 * kPerCu<FORM, TI>) void k_tiles(Args p) {
   constexpr bool kAcol = FORM != kNT, kBcol = FORM == kTN;
   constexpr int WJ = TJ / 64, WI = 8 / WJ;                        // wavefronts along i and j
   constexpr int FA = TI / WI / 16, FB = TJ / WJ / 16, FH = FA / 2;  // fragments of a wavefront
   static_assert(FB == 4, "mfma4");
   constexpr int LA = TI / 64, LB = TJ / 64;                   // loads of a wavefront per stage
   constexpr int kBytesA = TI * kStage, kBytes = kBytesA + TJ * kStage;
-  constexpr int BUFFERS = (147456 / kBytes);
+  constexpr int BUFFERS = 147456 / kPerCu<FORM, TI> / kBytes;
   constexpr int kPending = (BUFFERS - 2) * (LA + LB);
   constexpr int kC = kStage / Ty::kBytes;  // c of one stage
   __shared__ __align__(1024) uint8_t lds[BUFFERS * kBytes];
@@ -1159,12 +1167,12 @@ int compute_units() {
 
 template <class Ty, class Out, Form FORM, int TI, int TJ, bool ONCE>
 int launch_tiles(Args a, hipStream_t stream) {
-  const int cus = compute_units();
-  if (cus <= 0) return MEGAMOE_ERR_HIP;
+  const int most = compute_units() * kPerCu<FORM, TI>;
+  if (most <= 0) return MEGAMOE_ERR_HIP;
   const int64_t rows = FORM == kTN ? a.groups * ceil_div(a.n, TJ) : row_tiles(a.rows, a.groups, TJ, a.counts != nullptr);
   const int64_t total = rows * ceil_div(FORM == kTN ? a.k : a.n, TI);
   if (total > INT32_MAX) return MEGAMOE_ERR_UNSUPPORTED;
-  const int64_t grid = ceil_div(total < cus ? total : cus, 8) * 8;
+  const int64_t grid = ceil_div(total < most ? total : most, 8) * 8;
   hipLaunchKernelGGL((k_tiles<Ty, Out, FORM, TI, TJ, ONCE>), dim3((unsigned)grid), dim3(kThreads), 0, stream, a);
   return launched();
 }
@@ -1214,11 +1222,12 @@ double expected_tiles(const Args& a, const Load& l, int height) {
 double clamp01(double v) { return v < 0 ? 0 : v > 1 ? 1 : v; }
 
 // The tiled kernel for a product. Each size's time is its rounds of the GPU (not a whole number of
-// them costs about a third of one) times a tile's: its stages, and what its start and end cost in
-// stages. A stage of 256x128 takes 0.585 of one of 256x256 where the MFMAs decide (8192 cubed in
-// bf16: 204 us a round against 120) and 0.78 where the weights stream from memory (rows of a group
-// up to 128); one of 128x128 0.585 and 0.5 of 256x128's (7168 by 2048, 2 rows a group: 131 us a
-// round against 66).
+// them costs about a third of one, just more than the first 0.6) times a tile's: its stages, and what
+// its start and end cost in stages. A stage of 256x128 takes 0.585 of one of 256x256 where the MFMAs
+// decide (8192 cubed in bf16: 204 us a round against 120) and 0.78 where the weights stream from memory
+// (rows of a group up to 128); one of 128x128 0.585 and 0.5 of 256x128's (7168 by 2048, 2 rows a group:
+// 131 us a round against 66). Over 100 calls of 8 to 128 experts, 8 to 1024 uneven rows each, the size
+// that this takes is 1.0% slower than the fastest of the three in the geometric mean, 16% at most.
 //
 // ONCE loads the weights past the caches: they are not read again where a group's rows make up to
 // two tiles (225 of 256 experts hit, 7168 by 2048 in bf16: 1078 us without, 955 with it; 1024 rows a
@@ -1231,9 +1240,9 @@ int launch_rows(const Args& a, hipStream_t s) {
   const double kbytes = (double)a.k * Ty::kBytes, stages = ceil(kbytes / kStage);
   auto rounds = [&](int ti, int tj) {
     const double r = expected_tiles(a, l, tj) * ceil_div(a.n, ti) / cus;
-    return r <= 1 ? 1 : r + 0.3;
+    return r <= 1 ? 1 : fmax(r + 0.3, 1.6);
   };
-  const double unit_128 = 0.78 - 0.195 * clamp01((l.rows - 128) / 128);
+  const double unit_128 = 0.78 - 0.195 * clamp01((l.rows - 128) / 256);
   const double unit_64 = unit_128 * (0.5 + 0.085 * clamp01(l.rows / 128));
   const double large = rounds(256, 256) * (stages + 3), middle = rounds(256, 128) * unit_128 * (stages + 4.2);
   const double small = rounds(128, 128) * unit_64 * (stages + 5.4);
