@@ -354,7 +354,7 @@ def test_long_offsets():
 SIZES = {
     (256, 256, True): ([90, 110, 0, 200] * 16, 256, 520), (256, 256, False): ([3900, 4100], 256, 1032),
     (256, 128, True): ([4, 12, 0, 16] * 2, 256, 6144), (256, 128, False): ([4100, 3900], 256, 520),
-    (128, 128, True): ([2, 1, 5, 0] * 16, 256, 520), (128, 128, False): ([300, 500] * 4, 256, 1032),
+    (128, 128, True): ([2, 1, 5, 0] * 16, 256, 520), (128, 128, False): ([260, 340] * 4, 4096, 520),
 }
 
 
@@ -378,8 +378,9 @@ def _kernels(call):
 
 
 def _reached(kernel, kind, numbers, call):
-    """Whether ``call`` launches it. Demangled names can lose the first numbers, but not the last ones' order."""
-    return any(name == kernel and k == kind and n == numbers[len(numbers) - len(n):] for name, k, n in _kernels(call))
+    """Asserts that ``call`` launches it. Demangled names can lose the first numbers, but not the last ones' order."""
+    found = _kernels(call)
+    assert any(name == kernel and k == kind and n == numbers[len(numbers) - len(n):] for name, k, n in found), found
 
 
 @pytest.mark.parametrize("dtype", (BF16, FP16, torch.int8), ids=("bf16", "fp16", "int8"))
@@ -394,13 +395,13 @@ def test_every_tile_size_is_reached_and_exact(size, dtype):
         ws = torch.ones((len(counts), N), device=DEV)
         for out_dtype in (BF16, FP16, FP32):
             call = lambda: products.grouped_int8_mm(x, one, w, ws, c, out_dtype=out_dtype)  # noqa: E731
-            assert _reached("tiles", kind, size, call)
+            _reached("tiles", kind, size, call)
             _same(call(), _product(x, w, counts).float(), f"y {out_dtype}")
         return
     for transposed in (False, True):
         w = _whole((len(counts), K, N) if transposed else (len(counts), N, K), dtype, 151, most=3)
         call = lambda: products.grouped_mm(x, w, c, transposed=transposed)  # noqa: E731
-        assert _reached("tiles", kind, size, call)
+        _reached("tiles", kind, size, call)
         _same(call(), _product(x, w, counts, transposed), "y")
 
 
@@ -409,11 +410,11 @@ def test_the_other_kernels_are_reached():
     for dtype, kind in ((BF16, "Bf16"), (FP16, "Fp16")):
         for counts, K, N, strip in (([1] * 8, 2048, 768, (1, 1)), ([256], 2048, 768, (2, 2))):
             x, w, c = _whole((sum(counts), K), dtype, 152), _whole((len(counts), N, K), dtype, 153), _counts(counts)
-            assert _reached("strips", kind, strip, lambda: products.grouped_mm(x, w, c))
+            _reached("strips", kind, strip, lambda: products.grouped_mm(x, w, c))
             _same(products.grouped_mm(x, w, c), _product(x, w, counts), "y")
         for counts, K, N, size in (([30] * 20, 1024, 1000, (256, 256)), ([30, 5], 512, 520, (128, 128))):
             x, dy, c = _whole((sum(counts), K), dtype, 154), _whole((sum(counts), N), dtype, 155), _counts(counts)
-            assert _reached("tiles", kind, (*size, 0), lambda: products.grouped_mm_wgrad(dy, x, c))
+            _reached("tiles", kind, (*size, 0), lambda: products.grouped_mm_wgrad(dy, x, c))
             _same(products.grouped_mm_wgrad(dy, x, c), _wgrad(dy, x, counts), "dw")
         x, w, c = _whole((5, 33), dtype, 156), _whole((1, 9, 33), dtype, 157), _counts([5])
         names = _kernels(lambda: (products.grouped_mm(x, w, c), products.grouped_mm_wgrad(_whole((5, 9), dtype, 1), x, c)))
@@ -421,13 +422,13 @@ def test_the_other_kernels_are_reached():
     one = torch.ones(256, device=DEV)
     for M, strip in ((1, (1, 1)), (256, (2, 2))):
         x, w = _whole((M, 2048), torch.int8, 158), _whole((768, 2048), torch.int8, 159)
-        assert _reached("strips", "Int8", strip, lambda: products.int8_mm(x, one[:M], w, torch.ones(768, device=DEV)))
+        _reached("strips", "Int8", strip, lambda: products.int8_mm(x, one[:M], w, torch.ones(768, device=DEV)))
     for dtype in (BF16, FP16, FP32):
         wide = 16 // dtype.itemsize
         for chunks, kernel in ((64, (1, 1)), (128, (2, 1)), (256, (1, 0)), (512, (2, 0)), (1024, (4, 0)), (2048, (8, 0))):
             x = _whole((3, chunks * wide), dtype, 160)
-            assert _reached("quantize_int8", "", kernel, lambda: products.quantize_rows_int8(x))
-        assert _reached("quantize_int8_any", "", (), lambda: products.quantize_rows_int8(_whole((3, 33), dtype, 1)))
+            _reached("quantize_int8", "", kernel, lambda: products.quantize_rows_int8(x))
+        _reached("quantize_int8_any", "", (), lambda: products.quantize_rows_int8(_whole((3, 33), dtype, 1)))
 
 
 # ---------------------------------------------------------------------------------------

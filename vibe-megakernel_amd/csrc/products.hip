@@ -636,7 +636,7 @@ template <Form FORM, int TI>
 constexpr int kPerCu = FORM == kTN && TI == 128 ? 2 : 1;
 
 template <class Ty, class Out, Form FORM, int TI, int TJ, bool ONCE>
-__global__ __launch_bounds__(kThreads, 2 * kPerCu<FORM, TI>) void k_tiles(Args p) {
+__global__ __launch_bounds__(kThreads, (2 * kPerCu<FORM, TI>)) void k_tiles(Args p) {
   constexpr bool kAcol = FORM != kNT, kBcol = FORM == kTN;
   constexpr int WJ = TJ / 64, WI = 8 / WJ;                        // wavefronts along i and j
   constexpr int FA = TI / WI / 16, FB = TJ / WJ / 16, FH = FA / 2;  // fragments of a wavefront
