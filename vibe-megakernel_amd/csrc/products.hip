@@ -485,17 +485,18 @@ __device__ __forceinline__ i32x4 resource(const void* base, uint32_t bytes) {
 }
 
 // 16 bytes a lane into LDS (1024 consecutive ones from byte address `to`), from `base` + at +
-// along; zero from `bytes` on. ONCE: past the caches.
+// along; zero from `bytes` on. ONCE: past the caches. (Five wait states have to be between a
+// v_readfirstlane and a load that reads its SGPR; in here the compiler does not put them in.)
 template <bool ONCE>
 __device__ __forceinline__ void load_lds(uint32_t to, const uint8_t* base, uint32_t bytes, uint32_t at, uint32_t along) {
 #ifdef __HIP_DEVICE_COMPILE__
   if constexpr (ONCE)
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen nt lds"
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, %3 offen nt lds"
                  :
                  : "s"(uniform(to)), "v"(at), "s"(resource(base, bytes)), "s"(uniform(along))
                  : "memory", "m0");
   else
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
                  :
                  : "s"(uniform(to)), "v"(at), "s"(resource(base, bytes)), "s"(uniform(along))
                  : "memory", "m0");
@@ -505,7 +506,7 @@ __device__ __forceinline__ void load_lds(uint32_t to, const uint8_t* base, uint3
 // The same with 4 bytes a lane: `count` floats (up to 64, zero behind them).
 __device__ __forceinline__ void load_floats(uint32_t to, const float* base, int count) {
 #ifdef __HIP_DEVICE_COMPILE__
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dword %1, %2, 0 offen lds"
                :
                : "s"(uniform(to)), "v"((threadIdx.x & 63) * 4), "s"(resource(base, (uint32_t)max(count, 0) * 4))
                : "memory", "m0");
