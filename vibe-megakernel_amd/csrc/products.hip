@@ -40,6 +40,15 @@ constexpr int kMaxGroups = 1024;
       : "+v"(c[0]), "+v"(c[1]), "+v"(c[2]), "+v"(c[3])                                                           \
       : "v"(a), "v"(b[0]), "v"(b[1]), "v"(b[2]), "v"(b[3]))
 
+// One MFMA with the accumulator in AGPRs, for a wavefront that has a SIMD for itself; FIRST starts it
+// at zero. The operands come from LDS reads, so no wait states are needed; mfma_start() has those
+// behind what the compiler may copy between two steps.
+#define MEGAMOE_MFMA_ACC(name, c, a, b)                                     \
+  if constexpr (FIRST)                                                      \
+    asm(name " %0, %1, %2, 0" : "=a"(c) : "v"(a), "v"(b));                  \
+  else                                                                      \
+    asm(name " %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b))
+
 // What an element type of the operands brings: its accumulator and its 16x16 MFMA, whose lane l
 // holds row l % 16 and the 16 bytes at 16 * (l / 16) of both operands' c, and of the result rows
 // 4 * (l / 16) .. +3 (of A) in column l % 16 (of B).
@@ -54,6 +63,10 @@ struct Bf16 {
   static __device__ __forceinline__ void mfma4(Acc (&c)[4], i32x4 a, const i32x4 (&b)[4]) {
     MEGAMOE_MFMA4("v_mfma_f32_16x16x32_bf16", c, a, b);
   }
+  template <bool FIRST>
+  static __device__ __forceinline__ void mfma_acc(Acc& c, i32x4 a, i32x4 b) {
+    MEGAMOE_MFMA_ACC("v_mfma_f32_16x16x32_bf16", c, a, b);
+  }
 };
 struct Fp16 {
   using Elem = _Float16;
@@ -66,6 +79,10 @@ struct Fp16 {
   static __device__ __forceinline__ void mfma4(Acc (&c)[4], i32x4 a, const i32x4 (&b)[4]) {
     MEGAMOE_MFMA4("v_mfma_f32_16x16x32_f16", c, a, b);
   }
+  template <bool FIRST>
+  static __device__ __forceinline__ void mfma_acc(Acc& c, i32x4 a, i32x4 b) {
+    MEGAMOE_MFMA_ACC("v_mfma_f32_16x16x32_f16", c, a, b);
+  }
 };
 struct Int8 {
   using Elem = int8_t;
@@ -76,6 +93,10 @@ struct Int8 {
   }
   static __device__ __forceinline__ void mfma4(Acc (&c)[4], i32x4 a, const i32x4 (&b)[4]) {
     MEGAMOE_MFMA4("v_mfma_i32_16x16x64_i8", c, a, b);
+  }
+  template <bool FIRST>
+  static __device__ __forceinline__ void mfma_acc(Acc& c, i32x4 a, i32x4 b) {
+    MEGAMOE_MFMA_ACC("v_mfma_i32_16x16x64_i8", c, a, b);
   }
 };
 
@@ -347,23 +368,36 @@ __global__ __launch_bounds__(256) void k_wgrad_any(Args p) {
 // ---------------------------------------------------------------------------------------
 // The tiled product (16-byte aligned operands)
 //
-// A persistent workgroup of eight wavefronts per CU computes tiles of 256 (i) by TJ (j) outputs,
-// stage by stage of 128 bytes of c, each stage in two halves of 64 bytes. While one half's MFMAs
-// run from registers, the fragments of the next half are read from LDS: one operand's into
-// registers of its own, the other's in two parts of which the second takes the registers of
-// fragments that are done with. The second half of a stage is in registers before its first half
-// ends, so there the stage's buffer is free: one barrier a stage, at which no read is young,
-// and behind it the loads of the stage BUFFERS on, straight into LDS (64 KB or more in flight
-// per CU, no registers).
+// A persistent workgroup per CU computes tiles of TI (i) by TJ (j) outputs, stage by stage of c. The
+// loads of a stage go straight into LDS (no registers), BUFFERS stages ahead, 64 KB or more in flight
+// per CU; its fragments come to registers in halves of 64 bytes of c, one half ahead of the MFMAs.
 //
-// The stages of consecutive tiles follow each other without a gap: loads run over the tile's end,
-// so a tile's first stages are in LDS when the last tile's results are stored. (A tile has more
-// than BUFFERS stages; a short c is padded with zeros.)
+// 256x256: four wavefronts of 128x128 outputs each, one to a SIMD, with the accumulators in AGPRs.
+// They read a third less from LDS than eight of 128x64 (128 KB a stage of 128 bytes instead of 192,
+// at 128 bytes a clock against 2048 clocks of MFMAs, and 64 KB of loads written besides). A
+// wavefront alone has to issue everything between its own MFMAs: in the 16 clocks that one of them
+// takes three or four other instructions go, so reads and loads are dealt out singly between them.
+// (8192 cubed in bf16: 816 us with eight wavefronts, 800 with four and the reads and loads in bursts,
+// 755 so. The MFMAs alone are 457 us at 2.4 GHz, which the card does not hold under them: 1.8 to 2.0.)
+// A stage is 128 bytes of c where both operands have c contiguous (whole cache lines: half of them at a
+// time took 867 us instead of 755, and 173 instead of 135 for 128 experts of 256 rows, 2048 by 768),
+// and its loads go out in its second half, whose fragments are then in registers. It is 64 bytes in
+// four buffers instead of two where one has c across, and its loads go out in all of it (y = x w,
+// 8192 cubed: 910 us with eight wavefronts, 968 in stages of 128 bytes, 868 so).
 //
-// LDS layout. An operand with c contiguous: rows of 128 bytes, 16-byte chunk p of row r at
-// position p ^ (r % 8): one load instruction fills eight whole rows from full 128-byte lines,
-// and the MFMA's reads (16 rows of one chunk) fall into different banks. An operand with c
-// across: 64 rows (c) of all the tile's i or j, chunk p of row c at p ^ 2 f(c), f = c % 4 +
+// 256x128 and 128x128: eight wavefronts, two to a SIMD, that fill each other's pauses; a stage is 128
+// bytes. One operand's fragments come to registers of their own, the other's in two parts of which the
+// second takes the registers of fragments that are done with.
+//
+// Either way there is one barrier a stage, behind which the buffer read last is free for loads, and the
+// stages of consecutive tiles follow each other without a gap: loads run over the tile's end, so a
+// tile's first stages are in LDS when the last tile's results are stored. (A tile has more than
+// BUFFERS stages; a short c is padded with zeros.)
+//
+// LDS layout. An operand with c contiguous: rows of the stage's 128 (64) bytes, 16-byte chunk p of
+// row r at position p ^ (r % 8) (p ^ (r / 2 % 4)): one load instruction fills eight (sixteen) whole
+// rows, and the MFMA's reads (16 rows of one chunk) fall into different banks. An operand with c
+// across: 64 (32) rows (c) of all the tile's i or j, chunk p of row c at p ^ 2 f(c), f = c % 4 +
 // 4 (c / 8 % 2): the transposing reads (ds_read_b64_tr_b16: four c of 16 neighbours, for c = 8g ..
 // of the lane group g) fall into different banks as well.
 //
@@ -376,6 +410,7 @@ enum Form { kNT, kNN, kTN };  // y = x w^T, y = x w, dw = dy^T x
 constexpr int kThreads = 512, kStage = 128;
 
 typedef int i32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 // Until this wavefront's LDS reads have arrived and at most N of its loads into LDS are pending;
 // then the workgroup's wavefronts meet. Nothing moves across it.
@@ -398,6 +433,21 @@ __device__ __forceinline__ void mfma_done() {
   __builtin_amdgcn_sched_barrier(0);
 }
 
+// Wait states between a VALU result and an MFMA that reads it.
+__device__ __forceinline__ void mfma_start() {
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("s_nop 1");
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+// The value of an accumulator in an AGPR, read where it is used.
+template <class T>
+__device__ __forceinline__ T from_acc(T v) {
+  T r;
+  asm volatile("v_accvgpr_read_b32 %0, %1" : "=v"(r) : "a"(v));
+  return r;
+}
+
 // LDS at a byte address. The loads into LDS are inline asm without results (load_lds), so the
 // compiler counts the LDS reads alone and schedules them under the MFMAs by itself; the waits
 // for the loads are the phases' own.
@@ -413,13 +463,16 @@ __device__ __forceinline__ i32x2 lds_transposed(uint32_t at) {
 
 // One operand as this wavefront loads and reads it. COL: c across (else contiguous). L: the load
 // instructions of a wavefront per stage; load i fills the 1024 bytes wave + 8 i of the operand.
-template <bool COL, int L>
+// STEP: fragments between two of this wavefront.
+template <bool COL, int STAGE, int WAVES, int L, int STEP>
 struct Side {
-  static constexpr uint32_t kRow = COL ? 128 * L : 128;  // bytes of a row in LDS (COL: all 64 L columns)
-  uint32_t load;   // byte offset of the lane's 16 bytes of the first load from the tile's first row
-  uint32_t next;   // from one load of the wavefront to the next
-  uint32_t chunk;  // of `load`, the bytes along the contiguous dimension
-  uint32_t at[COL ? 1 : 2];  // LDS addresses of the lane's part of fragment 0
+  static constexpr uint32_t kRow = COL ? 2048 * WAVES * L / STAGE : STAGE;  // bytes of a row in LDS (COL: all of i or j)
+  // Loads in turn that differ in their chunk, where eight c are between two of them.
+  static constexpr int kKinds = COL && WAVES * 1024 / kRow % 16 ? 2 : 1;
+  uint32_t load[kKinds];   // byte offset of the lane's 16 bytes of the first load from the tile's first row
+  uint32_t next;           // from one load of the wavefront to the next
+  uint32_t chunk[kKinds];  // of `load`, the bytes along the contiguous dimension
+  uint32_t at[COL ? 1 : STAGE / 64];  // LDS addresses of the lane's part of fragment 0
 
   // `first`: the wavefront's first row; `base`: LDS address of the operand in buffer 0.
   __device__ __forceinline__ void init(uint32_t ld, int wave, int first, uint32_t base) {
@@ -427,19 +480,25 @@ struct Side {
     if constexpr (COL) {
       constexpr uint32_t kRows = 1024 / kRow, kLanes = 64 / kRows;  // of one load, of one row
       const uint32_t c = kRows * wave + lane / kLanes;
-      chunk = ((lane % kLanes) ^ (2 * ((c & 3) | ((c >> 1) & 4)))) * 16;
-      load = c * ld + chunk;
-      next = 8 * kRows * ld;
+#pragma unroll
+      for (uint32_t q = 0; q < kKinds; ++q) {
+        chunk[q] = ((lane % kLanes) ^ (2 * ((c & 3) | (((c >> 1) ^ (4 * q)) & 4)))) * 16;
+        load[q] = c * ld + chunk[q];
+      }
+      next = WAVES * kRows * ld;
       at[0] = base + (8 * g + ((lane & 15) >> 2)) * kRow +
               ((((uint32_t)(first >> 3) + ((lane & 3) >> 1)) ^ (2 * (((lane >> 2) & 3) | ((g & 1) << 2)))) << 4) +
               (lane & 1) * 8;
     } else {
-      chunk = ((lane & 7) ^ (lane >> 3)) * 16;
-      load = (8 * wave + (lane >> 3)) * ld + chunk;
-      next = 64 * ld;
+      // A load fills 1024 / STAGE rows; chunk p of row r is at p ^ swizzle(r).
+      constexpr uint32_t kChunks = STAGE / 16, kRows = 64 / kChunks;
+      const uint32_t row = lane / kChunks, r = lane & 15;
+      auto swizzle = [](uint32_t row) { return STAGE == 128 ? row & 7 : (row >> 1) & 3; };
+      chunk[0] = ((lane % kChunks) ^ swizzle(row)) * 16;
+      load[0] = (kRows * wave + row) * ld + chunk[0];
+      next = kRows * WAVES * ld;
 #pragma unroll
-      for (int s = 0; s < 2; ++s)
-        at[s] = base + ((uint32_t)first + (lane & 15)) * 128 + (((4 * s + g) ^ (lane & 7)) << 4);
+      for (int s = 0; s < STAGE / 64; ++s) at[s] = base + ((uint32_t)first + r) * STAGE + (((4 * s + g) ^ swizzle(r)) << 4);
     }
   }
   // The reads to another buffer, `by` bytes on (or back).
@@ -453,13 +512,19 @@ struct Side {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       if constexpr (COL) {
-        const uint32_t p = (at[0] ^ (32u * (BEGIN + i))) + 32 * kRow * s;
+        const uint32_t p = (at[0] ^ (32u * STEP * (BEGIN + i))) + 32 * kRow * s;
         const i32x2 lo = lds_transposed(p), hi = lds_transposed(p + 4 * kRow);
         f[i] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3);
       } else {
-        f[i] = lds_at<i32x4>(at[s] + 2048 * (BEGIN + i));
+        f[i] = lds_at<i32x4>(at[s] + 16 * STAGE * STEP * (BEGIN + i));
       }
     }
+  }
+  template <int I>
+  __device__ __forceinline__ void read_one(i32x4& f, int s) const {
+    i32x4 one[1];
+    read<I>(one, s);
+    f = one[0];
   }
 };
 
@@ -515,10 +580,38 @@ __device__ __forceinline__ void load_floats(uint32_t to, const float* base, int 
 
 // Load I of one operand's stage: `live` tells the lanes whose bytes exist, `bytes` the length of
 // the rows that do (the range check takes the sum of both offsets).
-template <int I, bool ONCE = false, class S>
-__device__ __forceinline__ void load_one(uint32_t to, int wave, const uint8_t* base, uint32_t bytes, const S& side,
-                                         bool live, uint32_t along) {
-  load_lds<ONCE>(to + (uint32_t)(wave + 8 * I) * 1024, base, bytes, live ? side.load : kOutside, along + I * side.next);
+template <int I, bool ONCE = false, bool COL, int STAGE, int WAVES, int L, int STEP>
+__device__ __forceinline__ void load_one(uint32_t to, int wave, const uint8_t* base, uint32_t bytes,
+                                         const Side<COL, STAGE, WAVES, L, STEP>& side, bool live, uint32_t along) {
+  load_lds<ONCE>(to + (uint32_t)(wave + WAVES * I) * 1024, base, bytes,
+                 live ? side.load[I % side.kKinds] : kOutside, along + I * side.next);
+}
+
+// The same load of a row of them, 4096 bytes of LDS and `next` of the operand apart: I of them, with
+// `along` starting one `next` in front. The resource, `to` and `along` come from settled().
+template <int I, bool ONCE>
+__device__ __forceinline__ void load_next(uint32_t to, i32x4 from, uint32_t at, uint32_t& along, uint32_t next) {
+#ifdef __HIP_DEVICE_COMPILE__
+  if constexpr (ONCE)
+    asm volatile("s_add_u32 m0, %1, %5\n\ts_add_u32 %0, %0, %4\n\tbuffer_load_dwordx4 %2, %3, %0 offen nt lds"
+                 : "+s"(along)
+                 : "s"(to), "v"(at), "s"(from), "s"(next), "i"(4096 * I)
+                 : "memory", "m0", "scc");
+  else
+    asm volatile("s_add_u32 m0, %1, %5\n\ts_add_u32 %0, %0, %4\n\tbuffer_load_dwordx4 %2, %3, %0 offen lds"
+                 : "+s"(along)
+                 : "s"(to), "v"(at), "s"(from), "s"(next), "i"(4096 * I)
+                 : "memory", "m0", "scc");
+#endif
+}
+// What load_next() takes, with the wait states between a v_readfirstlane and a load behind it.
+__device__ __forceinline__ void settled(i32x4& from, uint32_t& to, uint32_t& along, uint32_t& next) {
+#ifdef __HIP_DEVICE_COMPILE__
+  int f0 = uniform(from[0]), f1 = uniform(from[1]), f2 = uniform(from[2]), f3 = uniform(from[3]);
+  to = uniform(to), along = uniform(along), next = uniform(next);
+  asm volatile("s_nop 4" : "+s"(f0), "+s"(f1), "+s"(f2), "+s"(f3), "+s"(to), "+s"(along), "+s"(next));
+  from = i32x4{f0, f1, f2, f3};
+#endif
 }
 
 // Calls f(std::integral_constant<int, I>{}) for I = B .. E-1.
@@ -548,7 +641,7 @@ struct Table {
 // Fills the table; false if the counts do not fit the rows. Every thread of the workgroup calls it.
 __device__ bool make_table(Table& t, const Args& p, int height) {
   const int lane = threadIdx.x & 63;
-  for (int g = threadIdx.x; g < p.groups; g += kThreads) {
+  for (int g = threadIdx.x; g < p.groups; g += blockDim.x) {
     const int64_t v = p.counts ? p.counts[g] : p.rows;
     t.rows[g] = v < 0 || v > p.rows ? 0xffffffffu : (uint32_t)v;  // sums saturate at a value past the rows
   }
@@ -636,17 +729,28 @@ struct Work {
 template <Form FORM, int TI>
 constexpr int kPerCu = FORM == kTN && TI == 128 ? 2 : 1;
 
+// Wavefronts of a workgroup.
+template <int TI, int TJ>
+constexpr int kWaves = TI == 256 && TJ == 256 ? 4 : 8;
+
 template <class Ty, class Out, Form FORM, int TI, int TJ, bool ONCE>
-__global__ __launch_bounds__(kThreads, (2 * kPerCu<FORM, TI>)) void k_tiles(Args p) {
+__global__ __launch_bounds__((64 * kWaves<TI, TJ>), (kWaves<TI, TJ> / 4 * kPerCu<FORM, TI>)) void k_tiles(Args p) {
   constexpr bool kAcol = FORM != kNT, kBcol = FORM == kTN;
-  constexpr int WJ = TJ / 64, WI = 8 / WJ;                        // wavefronts along i and j
+  constexpr int WAVES = kWaves<TI, TJ>, THREADS = 64 * WAVES;
+  constexpr bool FOUR = WAVES == 4;
+  constexpr int WJ = FOUR ? 2 : TJ / 64, WI = WAVES / WJ;           // wavefronts along i and j
   constexpr int FA = TI / WI / 16, FB = TJ / WJ / 16, FH = FA / 2;  // fragments of a wavefront
-  static_assert(FB == 4, "mfma4");
-  constexpr int LA = TI / 64, LB = TJ / 64;                   // loads of a wavefront per stage
-  constexpr int kBytesA = TI * kStage, kBytes = kBytesA + TJ * kStage;
+  static_assert(FB == (FOUR ? 8 : 4), "mfma4");
+  // Four wavefronts take the fragments of j in turn, so that a tile of at most half the height has
+  // half of the fragments of each.
+  constexpr int STEP = FOUR ? WJ : 1;
+  constexpr int STAGE = FOUR && (kAcol || kBcol) ? 64 : kStage;     // bytes of c
+  constexpr int HALVES = STAGE / 64;
+  constexpr int LA = TI * STAGE / 1024 / WAVES, LB = TJ * STAGE / 1024 / WAVES;  // loads of a wavefront per stage
+  constexpr int kBytesA = TI * STAGE, kBytes = kBytesA + TJ * STAGE;
   constexpr int BUFFERS = 147456 / kPerCu<FORM, TI> / kBytes;
   constexpr int kPending = (BUFFERS - 2) * (LA + LB);
-  constexpr int kC = kStage / Ty::kBytes;  // c of one stage
+  constexpr int kC = STAGE / Ty::kBytes;  // c of one stage
   __shared__ __align__(1024) uint8_t lds[BUFFERS * kBytes];
   __shared__ Table table;
   // The int8 product's scales of two tiles' i and j, loaded with the tile's first stage.
@@ -663,7 +767,7 @@ __global__ __launch_bounds__(kThreads, (2 * kPerCu<FORM, TI>)) void k_tiles(Args
   if (!fits) {  // NaN everywhere
     const int64_t rows = FORM == kTN ? (int64_t)p.groups * p.n : p.rows;
     for (int64_t r = blockIdx.x; r < rows; r += gridDim.x)
-      for (int i = threadIdx.x; i < ni; i += kThreads) out[r * ldo + i] = (Out)__builtin_nanf("");
+      for (int i = threadIdx.x; i < ni; i += THREADS) out[r * ldo + i] = (Out)__builtin_nanf("");
     return;
   }
   const int used = uniform((int)table.rows[kMaxGroups]);
@@ -672,11 +776,13 @@ __global__ __launch_bounds__(kThreads, (2 * kPerCu<FORM, TI>)) void k_tiles(Args
   const int total = row_tiles * tiles_i;
   if (FORM != kTN && p.fill_rest)  // the last workgroups first: the ones that may have no tile
     for (int64_t r = used + (gridDim.x - 1 - blockIdx.x); r < p.rows; r += gridDim.x)
-      for (int i = threadIdx.x; i < ni; i += kThreads) out[r * ldo + i] = (Out)0.f;
+      for (int i = threadIdx.x; i < ni; i += THREADS) out[r * ldo + i] = (Out)0.f;
 
   const int64_t lda = (int64_t)Ty::kBytes * (FORM == kNT ? p.k : FORM == kNN ? p.n : p.ldx);
   const int64_t ldb = (int64_t)Ty::kBytes * (FORM == kTN ? p.ldy : p.ldx);
-  auto locate_work = [&](int tile) {
+  // A tile's stages: more than the buffers, and with four wavefronts, which take two in turn, even.
+  auto whole = [](int stages) { return FOUR && HALVES == 1 ? max(BUFFERS + 2, (stages + 1) / 2 * 2) : max(BUFFERS + 1, stages); };
+  auto locate_work = [&](int tile) __attribute__((always_inline)) {
     const int width = kBand * tiles_i, band = tile / width, in = tile % width;
     const int high = min(kBand, row_tiles - band * kBand);
     const int rt = band * kBand + in % high, it = in / high;
@@ -691,7 +797,7 @@ __global__ __launch_bounds__(kThreads, (2 * kPerCu<FORM, TI>)) void k_tiles(Args
       w.last = (int)lane_value(v, 1);
       w.a = p.x + (int64_t)w.first * lda + (int64_t)w.i0 * Ty::kBytes;
       w.b = p.w + (int64_t)w.first * ldb + (int64_t)w.j0 * Ty::kBytes;
-      w.stages = max(BUFFERS + 1, (w.last - w.first + kC - 1) / kC);
+      w.stages = whole((w.last - w.first + kC - 1) / kC);
     } else {
       const Tile t = table_tile(table, rt, TJ);
       w.group = t.group;
@@ -701,9 +807,9 @@ __global__ __launch_bounds__(kThreads, (2 * kPerCu<FORM, TI>)) void k_tiles(Args
       w.a = p.w + (size_t)w.group * p.n * p.k * Ty::kBytes +
             (FORM == kNT ? (int64_t)w.i0 * lda : (int64_t)w.i0 * Ty::kBytes);
       w.b = p.x + (int64_t)w.first * ldb;
-      w.stages = max(BUFFERS + 1, (p.k + kC - 1) / kC);
+      w.stages = whole((p.k + kC - 1) / kC);
     }
-    w.turn = FORM == kTN ? 0 : uniform((int)((uint32_t)w.group * kTurn % (uint32_t)w.stages));
+    w.turn = FORM == kTN ? 0 : uniform((int)((uint32_t)w.group * (kTurn * kStage / STAGE) % (uint32_t)w.stages));
     w.rows_a = uniform((uint32_t)min(p.n - w.i0, TI) * (uint32_t)lda);
     w.rows_b = uniform((uint32_t)(w.last - w.first) * (uint32_t)ldb);
     return w;
@@ -718,39 +824,43 @@ __global__ __launch_bounds__(kThreads, (2 * kPerCu<FORM, TI>)) void k_tiles(Args
   int stage = 0;                   // of `ahead`
   bool more = true;
 
-  Side<kAcol, LA> sa;
-  Side<kBcol, LB> sb;
+  Side<kAcol, STAGE, WAVES, LA, 1> sa;
+  Side<kBcol, STAGE, WAVES, LB, STEP> sb;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
   sa.init((uint32_t)lda, wave, wi * (TI / WI), lds0);
-  sb.init((uint32_t)ldb, wave, wj * (TJ / WJ), lds0 + kBytesA);
+  const int wave_j = FOUR ? 16 * wj : wj * (TJ / WJ);  // the wavefront's first j
+  sb.init((uint32_t)ldb, wave, wave_j, lds0 + kBytesA);
 
+  uint32_t row_bytes = (uint32_t)p.k * Ty::kBytes;  // (kept in a register, not loaded again in the loop)
+  asm("" : "+s"(row_bytes));
   // Load `i` of A's (or B's) loads at the load cursor, into buffer `buf`.
   auto at_stage = [&]() {
     const int s = stage + ahead.turn;
     return s >= ahead.stages && more ? s - ahead.stages : s;
   };
-  auto load_a = [&](auto i, int buf) {
-    if constexpr (Ty::kBytes == 1 && i.value == 0) {
-      if (stage == 0 && more) {
-        const uint32_t at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) float*)scales[ahead.place];
-        if (wave < TI / 64)
-          load_floats(at + 256 * wave, p.sw + (size_t)ahead.group * p.n + ahead.i0 + 64 * wave,
-                      min(p.n - ahead.i0 - 64 * wave, 64));
-        const int part = wave - (8 - TJ / 64);
-        if (part >= 0)
-          load_floats(at + 4 * TI + 256 * part, p.sx + ahead.first + 64 * part, min(ahead.last - ahead.first - 64 * part, 64));
-      }
+  auto load_scales = [&]() __attribute__((always_inline)) {
+    if (stage == 0 && more) {
+      const uint32_t at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) float*)scales[ahead.place];
+      if (wave < TI / 64)
+        load_floats(at + 256 * wave, p.sw + (size_t)ahead.group * p.n + ahead.i0 + 64 * wave,
+                    min(p.n - ahead.i0 - 64 * wave, 64));
+      const int part = wave - (WAVES - TJ / 64);
+      if (part >= 0)
+        load_floats(at + 4 * TI + 256 * part, p.sx + ahead.first + 64 * part, min(ahead.last - ahead.first - 64 * part, 64));
     }
+  };
+  auto load_a = [&](auto i, int buf) {
+    if constexpr (Ty::kBytes == 1 && i.value == 0) load_scales();
     const int stage = at_stage();
     const uint32_t to = lds0 + buf * kBytes;
     if constexpr (kAcol) {
       const int rows = (FORM == kTN ? ahead.last - ahead.first : p.k) - stage * kC;
       load_one<i.value, ONCE>(to, wave, ahead.a + (int64_t)stage * kC * lda,
                        more ? (uint32_t)min(max(rows, 0), kC) * (uint32_t)lda : 0u, sa,
-                       sa.chunk < (uint32_t)(ni - ahead.i0) * Ty::kBytes, 0u);
+                       sa.chunk[i.value % sa.kKinds] < (uint32_t)(ni - ahead.i0) * Ty::kBytes, 0u);
     } else {
       load_one<i.value, ONCE>(to, wave, ahead.a, ahead.rows_a, sa,
-                       (uint32_t)stage * kStage + sa.chunk < (uint32_t)p.k * Ty::kBytes, (uint32_t)stage * kStage);
+                       (uint32_t)stage * STAGE + sa.chunk[0] < row_bytes, (uint32_t)stage * STAGE);
     }
   };
   auto load_b = [&](auto i, int buf) {
@@ -760,14 +870,14 @@ __global__ __launch_bounds__(kThreads, (2 * kPerCu<FORM, TI>)) void k_tiles(Args
       const int rows = ahead.last - ahead.first - stage * kC;
       load_one<i.value>(to, wave, ahead.b + (int64_t)stage * kC * ldb,
                        more ? (uint32_t)min(max(rows, 0), kC) * (uint32_t)ldb : 0u, sb,
-                       sb.chunk < (uint32_t)(p.n - ahead.j0) * Ty::kBytes, 0u);
+                       sb.chunk[i.value % sb.kKinds] < (uint32_t)(p.n - ahead.j0) * Ty::kBytes, 0u);
     } else {
       load_one<i.value>(to, wave, ahead.b, ahead.rows_b, sb,
-                       (uint32_t)stage * kStage + sb.chunk < (uint32_t)p.k * Ty::kBytes, (uint32_t)stage * kStage);
+                       (uint32_t)stage * STAGE + sb.chunk[0] < row_bytes, (uint32_t)stage * STAGE);
     }
   };
   // The load cursor to the next stage, over the tile's end.
-  auto advance = [&]() {
+  auto advance = [&]() __attribute__((always_inline)) {
     if (++stage < ahead.stages || !more) return;
     stage = 0;
     tile = xcd_tile(++step, total);
@@ -781,76 +891,71 @@ __global__ __launch_bounds__(kThreads, (2 * kPerCu<FORM, TI>)) void k_tiles(Args
   };
 
   typename Ty::Acc acc[FA][FB];
-  // A's fragments of the lower and upper rows, one set more, and B's of two halves.
-  i32x4 x[FH], y[FH], z[FH], b0[FB], b1[FB];
-  auto clear = [&]() {
-#pragma unroll
-    for (int f = 0; f < FA; ++f)
-#pragma unroll
-      for (int t = 0; t < FB; ++t) acc[f][t] = typename Ty::Acc{0, 0, 0, 0};
-  };
-  // Fragments at .. at + n - 1 of a[], which are f0 .. of the tile, by b; the scheduler keeps it in
-  // one piece.
-  auto multiply = [&](const i32x4(&a)[FH], int f0, const i32x4(&b)[FB], int at, int n) {
-    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int f = at; f < at + n; ++f) Ty::mfma4(acc[f0 + f], a[f], b);
-    __builtin_amdgcn_sched_barrier(0);
-  };
-
   // Results: lane l has i = 4 (l / 16) .. +3 of a fragment at j = l % 16.
   auto store = [&]() {
     mfma_done();
     const int lane = opaque_lane();
     constexpr int kWide = 16 / (int)sizeof(Out);  // outputs of one store
     typedef Out OutN __attribute__((ext_vector_type(kWide)));
-    const bool wide = ldo % kWide == 0 && (uintptr_t)p.out % 16 == 0;
-    const int nj = FORM == kTN ? p.n : now.last - now.first;
-    Out* const base = FORM == kTN ? out + (size_t)now.group * p.n * p.k : out + (int64_t)now.first * ldo;
+    const bool wide = ldo % kWide == 0 && ni % kWide == 0 && (uintptr_t)p.out % 16 == 0;
+    const int nj = (FORM == kTN ? p.n : now.last - now.first) - now.j0;
+    // (Stores past the buffer, to kOutside, are dropped: no branches.)
+    const __amdgpu_buffer_rsrc_t to = __builtin_amdgcn_make_buffer_rsrc(
+        uniform(out + (FORM == kTN ? (size_t)now.group * p.n * p.k + (int64_t)now.j0 * ldo : (int64_t)now.first * ldo) + now.i0),
+        0, kOutside - 1, 0x00020000);
+    auto all = [&](auto wide) {
 #pragma unroll
-    for (int t = 0; t < FB; ++t) {
-      const int j = now.j0 + wj * (TJ / WJ) + 16 * t + (lane & 15);
-      float sx = 0.f;
-      if constexpr (Ty::kBytes == 1) sx = scales[now.place][TI + wj * (TJ / WJ) + 16 * t + (lane & 15)];
-      auto value = [&](int f, int e) {
-        if constexpr (Ty::kBytes == 1)
-          return scaled(acc[f][t][e], sx, scales[now.place][wi * (TI / WI) + 16 * f + 4 * (lane >> 4) + e]);
-        else
-          return acc[f][t][e];
-      };
-      auto put = [&](int i, OutN v) {
-        if (j >= nj) return;
-        Out* const row = base + (int64_t)j * ldo;
-        if (wide && i + kWide <= ni) {
-          *reinterpret_cast<OutN*>(row + i) = v;
-        } else {
+      for (int t = 0; t < FB; ++t) {
+        const int j = wave_j + 16 * STEP * t + (lane & 15);
+        float sx = 0.f;
+        if constexpr (Ty::kBytes == 1) sx = scales[now.place][TI + wave_j + 16 * STEP * t + (lane & 15)];
+        auto value = [&](int f, int e) {
+          const auto v = FOUR ? from_acc(acc[f][t][e]) : acc[f][t][e];
+          if constexpr (Ty::kBytes == 1)
+            return scaled(v, sx, scales[now.place][wi * (TI / WI) + 16 * f + 4 * (lane >> 4) + e]);
+          else
+            return v;
+        };
+        auto put = [&](int i, OutN v) {
+          const uint32_t at = ((uint32_t)j * (uint32_t)ldo + (uint32_t)i) * (uint32_t)sizeof(Out);
+          if constexpr (wide.value) {
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), to, j < nj && now.i0 + i < ni ? at : kOutside, 0, 0);
+          } else {
 #pragma unroll
-          for (int e = 0; e < kWide; ++e)
-            if (i + e < ni) row[i + e] = v[e];
-        }
-      };
+            for (int e = 0; e < kWide; ++e) {
+              const uint32_t one = j < nj && now.i0 + i + e < ni ? at + e * (uint32_t)sizeof(Out) : kOutside;
+              if constexpr (sizeof(Out) == 2)
+                __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, v[e]), to, one, 0, 0);
+              else
+                __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, v[e]), to, one, 0, 0);
+            }
+          }
+        };
 #pragma unroll
-      for (int f = 0; f < FA; f += kWide / 4) {
-        const int i = now.i0 + wi * (TI / WI) + 16 * f;
-        if constexpr (kWide == 4) {
-          put(i + 4 * (lane >> 4), OutN{(Out)value(f, 0), (Out)value(f, 1), (Out)value(f, 2), (Out)value(f, 3)});
-        } else {
-          // Two fragments' halves change places between neighbouring groups of 16 lanes, so that a
-          // lane has eight neighbours of one of them.
-          typedef Out Out2 __attribute__((ext_vector_type(2)));
-          uint32_t u[2][2];
+        for (int f = 0; f < FA; f += kWide / 4) {
+          const int i = wi * (TI / WI) + 16 * f;
+          if constexpr (kWide == 4) {
+            put(i + 4 * (lane >> 4), OutN{(Out)value(f, 0), (Out)value(f, 1), (Out)value(f, 2), (Out)value(f, 3)});
+          } else {
+            // Two fragments' halves change places between neighbouring groups of 16 lanes, so that a
+            // lane has eight neighbours of one of them.
+            typedef Out Out2 __attribute__((ext_vector_type(2)));
+            uint32_t u[2][2];
 #pragma unroll
-          for (int q = 0; q < 2; ++q)
+            for (int q = 0; q < 2; ++q)
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-              u[q][h] = __builtin_bit_cast(uint32_t, Out2{(Out)value(f + q, 2 * h), (Out)value(f + q, 2 * h + 1)});
-          const auto lo = __builtin_amdgcn_permlane16_swap(u[0][0], u[1][0], false, false);
-          const auto hi = __builtin_amdgcn_permlane16_swap(u[0][1], u[1][1], false, false);
-          const i32x4 all = {(int)lo[0], (int)hi[0], (int)lo[1], (int)hi[1]};
-          put(i + 16 * ((lane >> 4) & 1) + 8 * (lane >> 5), __builtin_bit_cast(OutN, all));
+              for (int h = 0; h < 2; ++h)
+                u[q][h] = __builtin_bit_cast(uint32_t, Out2{(Out)value(f + q, 2 * h), (Out)value(f + q, 2 * h + 1)});
+            const auto lo = __builtin_amdgcn_permlane16_swap(u[0][0], u[1][0], false, false);
+            const auto hi = __builtin_amdgcn_permlane16_swap(u[0][1], u[1][1], false, false);
+            const i32x4 all = {(int)lo[0], (int)hi[0], (int)lo[1], (int)hi[1]};
+            put(i + 16 * ((lane >> 4) & 1) + 8 * (lane >> 5), __builtin_bit_cast(OutN, all));
+          }
         }
       }
-    }
+    };
+    if (wide) all(std::true_type{});
+    else all(std::false_type{});
   };
 
   for (int i = 0; i < BUFFERS; ++i) {
@@ -858,10 +963,7 @@ __global__ __launch_bounds__(kThreads, (2 * kPerCu<FORM, TI>)) void k_tiles(Args
     static_for<0, LB>([&](auto l) { load_b(l, i); });
     advance();
   }
-  meet<(BUFFERS - 1) * (LA + LB)>();
-  sb.template read<0>(b0, 0);
-  sa.template read<0>(x, 0);
-  sa.template read<FH>(y, 0);
+  meet<(FOUR && HALVES == 1 ? BUFFERS - 2 : BUFFERS - 1) * (LA + LB)>();
   int buf = 0, last = 0;  // the buffer that is read, and the one before it
   auto next_buffer = [&]() {
     last = buf;
@@ -869,47 +971,192 @@ __global__ __launch_bounds__(kThreads, (2 * kPerCu<FORM, TI>)) void k_tiles(Args
     sa.move(buf == 0 ? -(BUFFERS - 1) * kBytes : kBytes);
     sb.move(buf == 0 ? -(BUFFERS - 1) * kBytes : kBytes);
   };
-  for (;;) {
-    clear();
-    const int nj = FORM == kTN ? p.n - now.j0 : now.last - now.first;
-    if (wj * (TJ / WJ) < nj) {
-      for (int left = now.stages; left > 0; --left) {
-        // First half of the stage: x, y and b0. The second half's fragments arrive in z, x and b1.
-        sb.template read<0>(b1, 1);
-        sa.template read<0>(z, 1);
-        multiply(x, 0, b0, 0, FH);
-        sa.template read<FH>(x, 1);
-        multiply(y, FH, b0, 0, FH);
-        meet<kPending>();
-        // Second half: z, x and b1. The next stage's first half arrives in x, y and b0.
-        next_buffer();
-        sb.template read<0>(b0, 0);
-        static_for<0, LA>([&](auto l) { load_a(l, last); });
-        sa.template read<FH>(y, 0);
-        multiply(x, FH, b1, 0, FH / 2);
-        static_for<0, LB>([&](auto l) { load_b(l, last); });
-        multiply(x, FH, b1, FH / 2, FH - FH / 2);
-        sa.template read<0>(x, 0);
-        multiply(z, 0, b1, 0, FH);
-        advance();
+  if constexpr (FOUR) {
+    // What is loaded of one operand at the load cursor.
+    struct Loads {
+      i32x4 from;
+      uint32_t to, along, next, at[2];
+    };
+    auto loads_a = [&](int buf) __attribute__((always_inline)) {
+      const int stage = at_stage();
+      Loads l;
+      if constexpr (kAcol) {
+        const int rows = (FORM == kTN ? ahead.last - ahead.first : p.k) - stage * kC;
+        l.from = resource(ahead.a + (int64_t)stage * kC * lda, more ? (uint32_t)min(max(rows, 0), kC) * (uint32_t)lda : 0u);
+        l.along = 0u - sa.next;
+#pragma unroll
+        for (int q = 0; q < sa.kKinds; ++q)
+          l.at[q] = sa.chunk[q] < (uint32_t)(ni - ahead.i0) * Ty::kBytes ? sa.load[q] : kOutside;
+      } else {
+        l.from = resource(ahead.a, ahead.rows_a);
+        l.along = (uint32_t)stage * STAGE - sa.next;
+        l.at[0] = (uint32_t)stage * STAGE + sa.chunk[0] < row_bytes ? sa.load[0] : kOutside;
       }
-    } else {
-      // No rows for this wavefront: it loads, and leaves the MFMAs to the one beside it (of a tile
-      // of at most half the height, every SIMD has one of either kind).
-      for (int left = now.stages; left > 0; --left) {
-        meet<kPending>();
-        next_buffer();
-        static_for<0, LA>([&](auto l) { load_a(l, last); });
-        static_for<0, LB>([&](auto l) { load_b(l, last); });
-        advance();
+      l.to = lds0 + buf * kBytes + wave * 1024;
+      l.next = sa.next;
+      settled(l.from, l.to, l.along, l.next);
+      return l;
+    };
+    auto loads_b = [&](int buf) __attribute__((always_inline)) {
+      const int stage = at_stage();
+      Loads l;
+      if constexpr (kBcol) {
+        const int rows = ahead.last - ahead.first - stage * kC;
+        l.from = resource(ahead.b + (int64_t)stage * kC * ldb, more ? (uint32_t)min(max(rows, 0), kC) * (uint32_t)ldb : 0u);
+        l.along = 0u - sb.next;
+#pragma unroll
+        for (int q = 0; q < sb.kKinds; ++q)
+          l.at[q] = sb.chunk[q] < (uint32_t)(p.n - ahead.j0) * Ty::kBytes ? sb.load[q] : kOutside;
+      } else {
+        l.from = resource(ahead.b, ahead.rows_b);
+        l.along = (uint32_t)stage * STAGE - sb.next;
+        l.at[0] = (uint32_t)stage * STAGE + sb.chunk[0] < row_bytes ? sb.load[0] : kOutside;
       }
-      sb.template read<0>(b0, 0);
-      sa.template read<0>(x, 0);
-      sa.template read<FH>(y, 0);
+      l.to = lds0 + buf * kBytes + kBytesA + wave * 1024;
+      l.next = sb.next;
+      settled(l.from, l.to, l.along, l.next);
+      return l;
+    };
+    // Read I of a stage's fragments, in the order of their use.
+    auto read = [&](auto i, auto wide, i32x4(&a)[FA], i32x4(&b)[FB], int s) __attribute__((always_inline)) {
+      constexpr int I = i.value;
+      if constexpr (I < 4) sb.template read_one<I>(b[I], s);
+      else if constexpr (I == 4) sa.template read_one<0>(a[0], s);
+      else if constexpr (!wide.value) sa.template read_one<I - 4>(a[I - 4], s);
+      else if constexpr (I < 9) sb.template read_one<I - 1>(b[I - 1], s);
+      else sa.template read_one<I - 8>(a[I - 8], s);
+    };
+    // One stage: a by b, while the next one's fragments arrive in an and bn (all of them for the
+    // `last` of a narrow tile, as the next tile may be a wide one), and the loads of the stage
+    // BUFFERS on are issued into this one's buffer: after every MFMA at most a few instructions, or
+    // the matrix pipe would run dry.
+    auto step_of = [&](auto half, auto first, auto wide, auto last_one, const i32x4(&a)[FA], const i32x4(&b)[FB], i32x4(&an)[FA],
+                        i32x4(&bn)[FB]) __attribute__((always_inline)) {
+      constexpr int NB = wide.value ? FB : FB / 2, MFMAS = FA * NB;
+      constexpr bool kAll = wide.value || last_one.value;
+      constexpr int READS = kAll ? FA + FB : FA + FB / 2;
+      // Of a stage of two halves, the first one's step reads on in its buffer, the other one's loads.
+      constexpr bool kReadOn = HALVES == 2 && half.value == 0, kMeet = HALVES == 1 || kReadOn;
+      Loads la, lb;
+      const int from = buf;
+      if constexpr (!kReadOn) next_buffer();
+      mfma_start();
+      static_for<0, MFMAS>([&](auto m) __attribute__((always_inline)) {
+        constexpr int M = m.value;
+        if constexpr (!kReadOn && M == 0) la = loads_a(from);
+        if constexpr (!kReadOn && M == MFMAS / 2) lb = loads_b(from);
+        if constexpr (!kReadOn && Ty::kBytes == 1 && M == 1) load_scales();
+        // Reads over the first half, loads over all of it.
+        static_for<(M < MFMAS / 2 ? READS * M / (MFMAS / 2) : READS), (M < MFMAS / 2 ? READS * (M + 1) / (MFMAS / 2) : READS)>(
+            [&](auto i) { read(i, std::bool_constant<kAll>{}, an, bn, kReadOn ? 1 : 0); });
+        constexpr int kEach = MFMAS / (LA + LB), L = M / kEach;
+        if constexpr (!kReadOn && M % kEach == kEach - 2) {
+          if constexpr (L < LA) load_next<L, ONCE>(la.to, la.from, la.at[L % sa.kKinds], la.along, la.next);
+          else load_next<L - LA, false>(lb.to, lb.from, lb.at[(L - LA) % sb.kKinds], lb.along, lb.next);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        Ty::template mfma_acc<first.value>(acc[M / NB][M % NB], a[M / NB], b[M % NB]);
+        __builtin_amdgcn_sched_barrier(0);
+      });
+      if constexpr (!kReadOn) advance();
+      if constexpr (kMeet) meet<kPending>();
+    };
+    i32x4 a0[FA], b0[FB], a1[FA], b1[FB];  // fragments of two stages
+    auto tile = [&](auto wide) __attribute__((always_inline)) {
+      constexpr std::false_type no;
+      constexpr std::true_type yes;
+      constexpr std::integral_constant<int, 0> lower;
+      constexpr std::integral_constant<int, HALVES - 1> upper;
+      step_of(lower, yes, wide, no, a0, b0, a1, b1);
+      step_of(upper, no, wide, no, a1, b1, a0, b0);
+      for (int left = now.stages * HALVES - 4; left > 0; left -= 2) {
+        step_of(lower, no, wide, no, a0, b0, a1, b1);
+        step_of(upper, no, wide, no, a1, b1, a0, b0);
+      }
+      step_of(lower, no, wide, no, a0, b0, a1, b1);
+      step_of(upper, no, wide, yes, a1, b1, a0, b0);
+    };
+    static_for<0, FA + FB>([&](auto i) { read(i, std::true_type{}, a0, b0, 0); });
+    if constexpr (HALVES == 1) meet<kPending>();
+    for (;;) {
+      const int nj = FORM == kTN ? p.n - now.j0 : now.last - now.first;
+      if (nj > TJ / 2) {
+        tile(std::true_type{});
+      } else {
+        tile(std::false_type{});
+        // The others' results are not stored: they need not outlive the loop.
+#pragma unroll
+        for (int f = 0; f < FA; ++f)
+#pragma unroll
+          for (int t = FB / 2; t < FB; ++t) asm("" : "=a"(acc[f][t]));
+      }
+      store();
+      if (!more) break;  // (the loads are BUFFERS stages ahead, within the next tile)
+      now = ahead;
     }
-    store();
-    if (!more) break;  // (the loads are BUFFERS + 1 stages ahead, within the next tile)
-    now = ahead;
+  } else {
+    // A's fragments of the lower and upper rows, one set more, and B's of two halves.
+    i32x4 x[FH], y[FH], z[FH], b0[FB], b1[FB];
+    auto clear = [&]() {
+#pragma unroll
+      for (int f = 0; f < FA; ++f)
+#pragma unroll
+        for (int t = 0; t < FB; ++t) acc[f][t] = typename Ty::Acc{0, 0, 0, 0};
+    };
+    // Fragments at .. at + n - 1 of a[], which are f0 .. of the tile, by b; the scheduler keeps it in
+    // one piece.
+    auto multiply = [&](const i32x4(&a)[FH], int f0, const i32x4(&b)[FB], int at, int n) {
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int f = at; f < at + n; ++f) Ty::mfma4(acc[f0 + f], a[f], b);
+      __builtin_amdgcn_sched_barrier(0);
+    };
+
+    sb.template read<0>(b0, 0);
+    sa.template read<0>(x, 0);
+    sa.template read<FH>(y, 0);
+    for (;;) {
+      clear();
+      const int nj = FORM == kTN ? p.n - now.j0 : now.last - now.first;
+      if (wj * (TJ / WJ) < nj) {
+        for (int left = now.stages; left > 0; --left) {
+          // First half of the stage: x, y and b0. The second half's fragments arrive in z, x and b1.
+          sb.template read<0>(b1, 1);
+          sa.template read<0>(z, 1);
+          multiply(x, 0, b0, 0, FH);
+          sa.template read<FH>(x, 1);
+          multiply(y, FH, b0, 0, FH);
+          meet<kPending>();
+          // Second half: z, x and b1. The next stage's first half arrives in x, y and b0.
+          next_buffer();
+          sb.template read<0>(b0, 0);
+          static_for<0, LA>([&](auto l) { load_a(l, last); });
+          sa.template read<FH>(y, 0);
+          multiply(x, FH, b1, 0, FH / 2);
+          static_for<0, LB>([&](auto l) { load_b(l, last); });
+          multiply(x, FH, b1, FH / 2, FH - FH / 2);
+          sa.template read<0>(x, 0);
+          multiply(z, 0, b1, 0, FH);
+          advance();
+        }
+      } else {
+        // No rows for this wavefront: it loads, and leaves the MFMAs to the one beside it (of a tile
+        // of at most half the height, every SIMD has one of either kind).
+        for (int left = now.stages; left > 0; --left) {
+          meet<kPending>();
+          next_buffer();
+          static_for<0, LA>([&](auto l) { load_a(l, last); });
+          static_for<0, LB>([&](auto l) { load_b(l, last); });
+          advance();
+        }
+        sb.template read<0>(b0, 0);
+        sa.template read<0>(x, 0);
+        sa.template read<FH>(y, 0);
+      }
+      store();
+      if (!more) break;  // (the loads are BUFFERS + 1 stages ahead, within the next tile)
+      now = ahead;
+    }
   }
   __builtin_amdgcn_s_waitcnt(0);  // loads into LDS may not outlive the workgroup
 }
@@ -1174,7 +1421,7 @@ int launch_tiles(Args a, hipStream_t stream) {
   const int64_t total = rows * ceil_div(FORM == kTN ? a.k : a.n, TI);
   if (total > INT32_MAX) return MEGAMOE_ERR_UNSUPPORTED;
   const int64_t grid = ceil_div(total < most ? total : most, 8) * 8;
-  hipLaunchKernelGGL((k_tiles<Ty, Out, FORM, TI, TJ, ONCE>), dim3((unsigned)grid), dim3(kThreads), 0, stream, a);
+  hipLaunchKernelGGL((k_tiles<Ty, Out, FORM, TI, TJ, ONCE>), dim3((unsigned)grid), dim3(64 * kWaves<TI, TJ>), 0, stream, a);
   return launched();
 }
 
