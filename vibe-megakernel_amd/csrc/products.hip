@@ -754,7 +754,7 @@ __global__ __launch_bounds__((64 * kWaves<TI, TJ>), (kWaves<TI, TJ> / 4 * kPerCu
   __shared__ __align__(1024) uint8_t lds[BUFFERS * kBytes];
   __shared__ Table table;
   // The int8 product's scales of two tiles' i and j, loaded with the tile's first stage.
-  __shared__ float scales[2][Ty::kBytes == 1 ? TI + TJ : 1];
+  __shared__ __align__(16) float scales[2][Ty::kBytes == 1 ? TI + TJ : 1];
 
   const int wave = uniform((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int wi = wave % WI, wj = wave / WI;
@@ -903,6 +903,12 @@ __global__ __launch_bounds__((64 * kWaves<TI, TJ>), (kWaves<TI, TJ> / 4 * kPerCu
     const __amdgpu_buffer_rsrc_t to = __builtin_amdgcn_make_buffer_rsrc(
         uniform(out + (FORM == kTN ? (size_t)now.group * p.n * p.k + (int64_t)now.j0 * ldo : (int64_t)now.first * ldo) + now.i0),
         0, kOutside - 1, 0x00020000);
+    f32x4 sw[FA];
+    if constexpr (Ty::kBytes == 1) {
+#pragma unroll
+      for (int f = 0; f < FA; ++f)
+        sw[f] = *reinterpret_cast<const f32x4*>(&scales[now.place][wi * (TI / WI) + 16 * f + 4 * (lane >> 4)]);
+    }
     auto all = [&](auto wide) {
 #pragma unroll
       for (int t = 0; t < FB; ++t) {
@@ -912,7 +918,7 @@ __global__ __launch_bounds__((64 * kWaves<TI, TJ>), (kWaves<TI, TJ> / 4 * kPerCu
         auto value = [&](int f, int e) {
           const auto v = FOUR ? from_acc(acc[f][t][e]) : acc[f][t][e];
           if constexpr (Ty::kBytes == 1)
-            return scaled(v, sx, scales[now.place][wi * (TI / WI) + 16 * f + 4 * (lane >> 4) + e]);
+            return scaled(v, sx, sw[f][e]);
           else
             return v;
         };
