@@ -405,6 +405,35 @@ def test_every_tile_size_is_reached_and_exact(size, dtype):
         _same(call(), _product(x, w, counts, transposed), "y")
 
 
+@pytest.mark.parametrize("dtype", (BF16, FP16, torch.int8), ids=("bf16", "fp16", "int8"))
+@pytest.mark.parametrize("size", SIZES, ids=lambda s: f"{s[0]}x{s[1]}{'-once' if s[2] else ''}")
+def test_tiles_store_rows_that_are_not_aligned(size, dtype):
+    """An odd N, and results whose rows start anywhere; what lies between them stays."""
+    counts, K, N = SIZES[size]
+    N, R = N + 3, sum(counts)
+    _log(f"{size} {dtype}: {R} rows of {len(counts)} experts, K={K} N={N}")
+    x, c = _whole((R, K), dtype, 160, most=3), _counts(counts)
+    w = _whole((len(counts), N, K), dtype, 161, most=3)
+    out = torch.full((R, N + 6), 7.0, dtype=BF16 if dtype == torch.int8 else dtype, device=DEV)
+    if dtype == torch.int8:
+        products.grouped_int8_mm(x, torch.ones(R, device=DEV), w, torch.ones((len(counts), N), device=DEV), c,
+                                 out=out[:, 1:N + 1])
+    else:
+        products.grouped_mm(x, w, c, out=out[:, 1:N + 1])
+    _same(out[:, 1:N + 1], _product(x, w, counts).float() if dtype == torch.int8 else _product(x, w, counts), "y")
+    assert bool((out[:, 0] == 7).all()) and bool((out[:, N + 1:] == 7).all())
+
+
+def test_weight_gradient_tiles_store_anywhere():
+    for counts, K, N in (([30] * 20, 1024, 1000), ([30, 5], 512, 520), ([700, 0, 3] * 3, 2048, 776)):
+        x, dy, c = _whole((sum(counts), K), BF16, 162), _whole((sum(counts), N), BF16, 163), _counts(counts)
+        flat = torch.full((len(counts) * N * K + 2,), 7.0, dtype=BF16, device=DEV)
+        dw = flat[1:-1].view(len(counts), N, K)
+        products.grouped_mm_wgrad(dy, x, c, out=dw)
+        _same(dw, _wgrad(dy, x, counts), "dw")
+        assert flat[0] == 7 and flat[-1] == 7
+
+
 def test_the_other_kernels_are_reached():
     """Strips of both sizes, both tile sizes of the weights' gradient, the kernels of any alignment."""
     for dtype, kind in ((BF16, "Bf16"), (FP16, "Fp16")):

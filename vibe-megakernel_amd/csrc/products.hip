@@ -929,11 +929,12 @@ __global__ __launch_bounds__((64 * kWaves<TI, TJ>), (kWaves<TI, TJ> / 4 * kPerCu
           } else {
 #pragma unroll
             for (int e = 0; e < kWide; ++e) {
+              const Out element = v[e];  // (__builtin_bit_cast of v[e] itself takes v[0])
               const uint32_t one = j < nj && now.i0 + i + e < ni ? at + e * (uint32_t)sizeof(Out) : kOutside;
               if constexpr (sizeof(Out) == 2)
-                __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, v[e]), to, one, 0, 0);
+                __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, element), to, one, 0, 0);
               else
-                __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, v[e]), to, one, 0, 0);
+                __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, element), to, one, 0, 0);
             }
           }
         };
