@@ -4,6 +4,7 @@ declares, and every bad argument is refused before anything reaches a GPU."""
 from __future__ import annotations
 
 import ctypes
+import json
 import re
 import subprocess
 from pathlib import Path
@@ -12,6 +13,7 @@ import pytest
 import torch
 
 from vibe_megakernel_amd import _lib, products
+from vibe_megakernel_amd import build as pkg_build
 
 HEADER = Path(__file__).resolve().parent.parent / "include" / "megamoe_products.h"
 FAKE = 4096  # a pointer that is never followed: the checks answer first
@@ -118,3 +120,16 @@ def test_row_strides():
     assert products._stride(t.t()) is None and products._stride(t[:1].expand(6, 10)) is None
     a, b = products._extent(t[1:3, 2:5])
     assert a == t.data_ptr() + 4 * 12 and b == t.data_ptr() + 4 * 25
+
+
+def test_no_kernel_spills():
+    """The compiler's report of the built library: registers of the products that go to memory cost more than the
+    results show, and the four wavefronts of the 256x256 tiles hold 256 AGPRs each without one to spare."""
+    if not pkg_build.REPORT.exists():
+        pytest.skip("no resource report: the library has not been built here")
+    report = json.loads(pkg_build.REPORT.read_text())
+    names = [n for n in report if re.search(r"k_(tiles|strips|product_any|wgrad_any|quantize_int8)", n)]
+    assert len(names) >= 60
+    for n in names:
+        assert report[n]["scratch_bytes"] == 0 and report[n]["vgpr_spills"] == 0, (n, report[n])
+        assert report[n]["lds_bytes"] <= 160 * 1024, (n, report[n])

@@ -1478,11 +1478,11 @@ double clamp01(double v) { return v < 0 ? 0 : v > 1 ? 1 : v; }
 
 // The tiled kernel for a product. Each size's time is its rounds of the GPU (not a whole number of
 // them costs about a third of one, just more than the first 0.6) times a tile's: its stages, and what
-// its start and end cost in stages. A stage of 256x128 takes 0.585 of one of 256x256 where the MFMAs
-// decide (8192 cubed in bf16: 204 us a round against 120) and 0.78 where the weights stream from memory
+// its start and end cost in stages. A stage of 256x128 takes 0.63 of one of 256x256 where the MFMAs
+// decide (8192 cubed in bf16: 189 us a round against 120) and 0.78 where the weights stream from memory
 // (rows of a group up to 128); one of 128x128 0.585 and 0.5 of 256x128's (7168 by 2048, 2 rows a group:
 // 131 us a round against 66). Over 100 calls of 8 to 128 experts, 8 to 1024 uneven rows each, the size
-// that this takes is 1.0% slower than the fastest of the three in the geometric mean, 16% at most.
+// that this takes is 0.6% slower than the fastest of the three in the geometric mean, 12% at most.
 //
 // ONCE loads the weights past the caches: they are not read again where a group's rows make up to
 // two tiles (225 of 256 experts hit, 7168 by 2048 in bf16: 1078 us without, 955 with it; 1024 rows a
@@ -1497,7 +1497,7 @@ int launch_rows(const Args& a, hipStream_t s) {
     const double r = expected_tiles(a, l, tj) * ceil_div(a.n, ti) / cus;
     return r <= 1 ? 1 : fmax(r + 0.3, 1.6);
   };
-  const double unit_128 = 0.78 - 0.195 * clamp01((l.rows - 128) / 256);
+  const double unit_128 = 0.78 - 0.15 * clamp01((l.rows - 128) / 256);
   const double unit_64 = unit_128 * (0.5 + 0.085 * clamp01(l.rows / 128));
   const double large = rounds(256, 256) * (stages + 3), middle = rounds(256, 128) * unit_128 * (stages + 4.2);
   const double small = rounds(128, 128) * unit_64 * (stages + 5.4);
