@@ -414,14 +414,44 @@ def test_tiles_store_rows_that_are_not_aligned(size, dtype):
     _log(f"{size} {dtype}: {R} rows of {len(counts)} experts, K={K} N={N}")
     x, c = _whole((R, K), dtype, 160, most=3), _counts(counts)
     w = _whole((len(counts), N, K), dtype, 161, most=3)
-    out = torch.full((R, N + 6), 7.0, dtype=BF16 if dtype == torch.int8 else dtype, device=DEV)
-    if dtype == torch.int8:
-        products.grouped_int8_mm(x, torch.ones(R, device=DEV), w, torch.ones((len(counts), N), device=DEV), c,
-                                 out=out[:, 1:N + 1])
-    else:
-        products.grouped_mm(x, w, c, out=out[:, 1:N + 1])
-    _same(out[:, 1:N + 1], _product(x, w, counts).float() if dtype == torch.int8 else _product(x, w, counts), "y")
-    assert bool((out[:, 0] == 7).all()) and bool((out[:, N + 1:] == 7).all())
+    for out_dtype in (BF16, FP16, FP32) if dtype == torch.int8 else (dtype,):
+        out = torch.full((R, N + 6), 7.0, dtype=out_dtype, device=DEV)
+        if dtype == torch.int8:
+            products.grouped_int8_mm(x, torch.ones(R, device=DEV), w, torch.ones((len(counts), N), device=DEV), c,
+                                     out_dtype=out_dtype, out=out[:, 1:N + 1])
+        else:
+            products.grouped_mm(x, w, c, out=out[:, 1:N + 1])
+        want = _product(x, w, counts)
+        _same(out[:, 1:N + 1], want.float() if dtype == torch.int8 else want, f"y {out_dtype}")
+        assert bool((out[:, 0] == 7).all()) and bool((out[:, N + 1:] == 7).all())
+
+
+@pytest.mark.parametrize("dtype", (BF16, FP16), ids=("bf16", "fp16"))
+@pytest.mark.parametrize("size", SIZES, ids=lambda s: f"{s[0]}x{s[1]}{'-once' if s[2] else ''}")
+def test_tiles_read_strided_rows_and_nothing_between(size, dtype):
+    """Rows in a wider tensor whose other columns, and rows behind the last expert's, are NaN."""
+    counts, K, N = SIZES[size]
+    S = sum(counts)
+    _log(f"{size} {dtype}: {S} rows of {len(counts)} experts, K={K} N={N}")
+
+    def within(values):
+        wide = torch.full((S + 5, values.shape[1] + 24), float("nan"), dtype=dtype, device=DEV)
+        wide[:S, 8:-16] = values
+        return wide[:, 8:-16]
+
+    x, dy, c = _whole((S, K), dtype, 164, most=3), _whole((S, N), dtype, 165, most=3), _counts(counts)
+    w = _whole((len(counts), N, K), dtype, 166, most=3)
+    y = products.grouped_mm(within(x), w, c)
+    _same(y[:S], _product(x, w, counts), "y")
+    assert bool((y[S:] == 0).all())
+    dx = torch.full((S + 5, K), 7.0, dtype=dtype, device=DEV)
+    products.grouped_mm(within(dy), w, c, transposed=True, out=dx)
+    _same(dx[:S], _product(dy, w, counts, True), "dx")
+    assert bool((dx[S:] == 7).all())
+    _same(products.grouped_mm_wgrad(within(dy), within(x), c), _wgrad(dy, x, counts), "dw")
+    c[-1] += 6  # one row more than there are
+    assert bool(products.grouped_mm(within(x), w, c).isnan().all())
+    assert bool(products.grouped_mm_wgrad(within(dy), within(x), c).isnan().all())
 
 
 def test_weight_gradient_tiles_store_anywhere():
